@@ -534,6 +534,13 @@ int do_fwd(const fkda_fwd_params* p, void* cuda_stream, bool fit) {
 }  // namespace
 
 namespace fkda {
+int set_error(int code, const char* fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(g_err, sizeof(g_err), fmt, ap);
+  va_end(ap);
+  return code;
+}
 int fwd_within(const fkda_fwd_params* p, void* cuda_stream) { return do_fwd(p, cuda_stream, true); }
 }  // namespace fkda
 

@@ -1,0 +1,94 @@
+// Parameter blocks and host checks that the operators round the recurrence share (short convolution, selective scan, norms).
+#pragma once
+#include "fkda_common.cuh"
+
+namespace fkda {
+
+// A [B][T][...] tensor whose tokens are `token` elements apart and whose batch rows `batch`.
+struct Rows {
+  int64_t batch, token;
+};
+
+struct ConvParams {
+  const __nv_bfloat16* x;
+  const void* weight;
+  const void* bias;
+  __nv_bfloat16* out;
+  const __nv_bfloat16* initial_state;
+  __nv_bfloat16* final_state;
+  const int64_t* cu_seqlens;
+  Rows xs, os;
+  int64_t T;                // tokens of a sequence, or of the packed batch
+  int C;
+  int N;
+  int tile;                 // tokens of a block
+  int tiles;                // ... of a sequence, or of the packed batch
+  int silu;
+};
+cudaError_t launch_short_conv(ConvParams p, int width, bool weight_fp32, cudaStream_t stream);
+
+struct SsmParams {
+  const __nv_bfloat16* x;
+  const __nv_bfloat16* dt;
+  const __nv_bfloat16* Bm;
+  const __nv_bfloat16* Cm;
+  __nv_bfloat16* out;
+  const float* A_log;
+  const float* dt_bias;
+  const float* D;
+  const void* initial_state;
+  void* final_state;
+  const int64_t* cu_seqlens;
+  Rows xs, dts, bs, cs, os;
+  int64_t T;
+  int H, P, G, Ns, N;
+  int state_fp32;
+};
+cudaError_t launch_ssm_step(const SsmParams& p, cudaStream_t stream);
+
+struct GatedNormParams {
+  const __nv_bfloat16* x;
+  const __nv_bfloat16* gate;
+  const void* weight;
+  __nv_bfloat16* out;
+  Rows xs, gs, os;
+  int64_t rows;             // B T H
+  int64_t T;
+  int H, D;
+  float eps;
+  int per_head;
+};
+cudaError_t launch_gated_norm(const GatedNormParams& p, bool weight_fp32, bool silu, bool gate_first, cudaStream_t stream);
+
+struct AddNormParams {
+  const __nv_bfloat16* x;
+  const void* residual;
+  const void* weight;
+  __nv_bfloat16* out;
+  void* residual_out;
+  Rows xs, rs, os, ros;
+  int64_t rows;             // B T
+  int64_t T;
+  int D;
+  float scale, eps;
+};
+cudaError_t launch_add_norm(const AddNormParams& p, bool weight_fp32, bool residual_fp32, cudaStream_t stream);
+
+// The library's error message of this thread (fkda_last_error); returns `code`.
+int set_error(int code, const char* fmt, ...);
+
+// Eight consecutive weights as fp32.
+template <bool kFp32>
+__device__ __forceinline__ void load8(const void* base, int64_t at, float (&w)[8]) {
+  if constexpr (kFp32) {
+    const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(base) + at);
+    const float4 a = __ldg(q), b = __ldg(q + 1);
+    w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w; w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
+  } else {
+    unpack8(__ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(base) + at)), w);
+  }
+}
+// 1 / (1 + e^-x) to fp32 accuracy (the tanh approximation has an absolute error that small values do not bear)
+__device__ __forceinline__ float sigmoid_exact(float x) { return __fdividef(1.f, 1.f + ex2f(-kLog2e * x)); }
+
+}  // namespace fkda

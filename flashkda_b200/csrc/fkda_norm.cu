@@ -1,0 +1,217 @@
+// Root-mean-square norms before and after the recurrence's block: with its gate, and with the residual stream.
+//
+//   gated_norm   out = x / rms(x) w a(g)  or  (x a) / rms(x a) w,  a = sigmoid(g) or g sigmoid(g)
+//   add_norm     h = residual + scale x -> residual_out;  out = h / rms(h) w
+//
+// One pass: a row lives in the registers of the threads that share it, eight elements (16 bytes of bf16) at a time, from its loads to its
+// stores; the sum of squares is fp32.  Rows of up to 1024 elements are shared by 8 to 32 lanes of a warp, longer ones by a block.
+#include "fkda_layer.cuh"
+
+namespace fkda {
+namespace norm {
+
+// Sum over the `lanes` threads that share a row (a power of two up to 32), or over the block.
+template <bool kBlock>
+__device__ __forceinline__ float row_sum(float x, int lanes, float* scratch) {
+  const int width = kBlock ? 32 : lanes;
+  for (int d = width >> 1; d > 0; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+  if constexpr (kBlock) {
+    const int warps = blockDim.x >> 5;
+    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = x;
+    __syncthreads();
+    x = 0.f;
+    for (int i = 0; i < warps; ++i) x += scratch[i];
+  }
+  return x;
+}
+
+// Where the row that this thread works on starts, and which eight-element pieces of it are its own: lane, lane + lanes, ...
+struct Place {
+  int64_t row;
+  int lane, lanes;
+  bool live;
+};
+template <bool kBlock>
+__device__ __forceinline__ Place place(int64_t rows, int lanes) {
+  Place w;
+  if constexpr (kBlock) {
+    w.row = blockIdx.x;
+    w.lane = threadIdx.x;
+    w.lanes = blockDim.x;
+  } else {
+    const int per = blockDim.x / lanes;
+    w.row = static_cast<int64_t>(blockIdx.x) * per + threadIdx.x / lanes;
+    w.lane = threadIdx.x % lanes;
+    w.lanes = lanes;
+  }
+  w.live = w.row < rows;
+  if (!w.live) w.row = rows - 1;               // (takes part in the sums, stores nothing)
+  return w;
+}
+__device__ __forceinline__ int64_t at_token(const Rows& s, int64_t token, int64_t T) {
+  const int64_t b = token / T;
+  return b * s.batch + (token - b * T) * s.token;
+}
+
+template <bool kBlock, int V, bool kWFp32, bool kSilu, bool kFirst>
+__global__ void gated_norm_kernel(const GatedNormParams p, int lanes) {
+  __shared__ float scratch[32];
+  grid_dependency_wait();
+  const Place at = place<kBlock>(p.rows, lanes);
+  const int64_t token = at.row / p.H;
+  const int h = static_cast<int>(at.row - token * p.H), pieces = p.D / 8;
+  const __nv_bfloat16* x = p.x + at_token(p.xs, token, p.T) + static_cast<int64_t>(h) * p.D;
+  const __nv_bfloat16* g = p.gate + at_token(p.gs, token, p.T) + static_cast<int64_t>(h) * p.D;
+  uint4 xw[V], gw[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int c = at.lane + i * at.lanes;
+    xw[i] = gw[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (c < pieces) {
+      xw[i] = *reinterpret_cast<const uint4*>(x + 8 * c);
+      gw[i] = *reinterpret_cast<const uint4*>(g + 8 * c);
+    }
+  }
+  float u[V][8], sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    unpack8(xw[i], u[i]);
+    if constexpr (kFirst) {
+      float a[8];
+      unpack8(gw[i], a);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) u[i][e] *= kSilu ? a[e] * sigmoid_exact(a[e]) : sigmoid_exact(a[e]);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum = fmaf(u[i][e], u[i][e], sum);
+  }
+  const float r = rsqrtf(row_sum<kBlock>(sum, lanes, scratch) / static_cast<float>(p.D) + p.eps);
+  if (!at.live) return;
+  __nv_bfloat16* out = p.out + at_token(p.os, token, p.T) + static_cast<int64_t>(h) * p.D;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int c = at.lane + i * at.lanes;
+    if (c >= pieces) break;
+    float w[8], a[8];
+    load8<kWFp32>(p.weight, (p.per_head ? static_cast<int64_t>(h) * p.D : 0) + 8 * c, w);
+    if constexpr (!kFirst) unpack8(gw[i], a);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      u[i][e] *= r * w[e];
+      if constexpr (!kFirst) u[i][e] *= kSilu ? a[e] * sigmoid_exact(a[e]) : sigmoid_exact(a[e]);
+    }
+    *reinterpret_cast<uint4*>(out + 8 * c) = pack8(u[i]);
+  }
+}
+
+template <bool kBlock, int V, bool kWFp32, bool kRFp32>
+__global__ void add_norm_kernel(const AddNormParams p, int lanes) {
+  __shared__ float scratch[32];
+  grid_dependency_wait();
+  const Place at = place<kBlock>(p.rows, lanes);
+  const int pieces = p.D / 8;
+  const __nv_bfloat16* x = p.x + at_token(p.xs, at.row, p.T);
+  const int64_t from = at_token(p.rs, at.row, p.T);
+  uint4 xw[V];
+  float u[V][8], sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int c = at.lane + i * at.lanes;
+    xw[i] = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) u[i][e] = 0.f;
+    if (c < pieces) {
+      xw[i] = *reinterpret_cast<const uint4*>(x + 8 * c);
+      if constexpr (kRFp32) {
+        const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p.residual) + from + 8 * c);
+        const float4 a = q[0], b = q[1];
+        u[i][0] = a.x; u[i][1] = a.y; u[i][2] = a.z; u[i][3] = a.w; u[i][4] = b.x; u[i][5] = b.y; u[i][6] = b.z; u[i][7] = b.w;
+      } else {
+        unpack8(*reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.residual) + from + 8 * c), u[i]);
+      }
+    }
+  }
+  const int64_t to = at_token(p.ros, at.row, p.T);
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int c = at.lane + i * at.lanes;
+    float xf[8];
+    unpack8(xw[i], xf);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      u[i][e] = fmaf(p.scale, xf[e], u[i][e]);
+      sum = fmaf(u[i][e], u[i][e], sum);
+    }
+    if (c < pieces && at.live) {
+      if constexpr (kRFp32) {
+        float4* q = reinterpret_cast<float4*>(static_cast<float*>(p.residual_out) + to + 8 * c);
+        q[0] = make_float4(u[i][0], u[i][1], u[i][2], u[i][3]);
+        q[1] = make_float4(u[i][4], u[i][5], u[i][6], u[i][7]);
+      } else {
+        *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.residual_out) + to + 8 * c) = pack8(u[i]);
+      }
+    }
+  }
+  const float r = rsqrtf(row_sum<kBlock>(sum, lanes, scratch) / static_cast<float>(p.D) + p.eps);
+  if (!at.live) return;
+  __nv_bfloat16* out = p.out + at_token(p.os, at.row, p.T);
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int c = at.lane + i * at.lanes;
+    if (c >= pieces) break;
+    float w[8];
+    load8<kWFp32>(p.weight, 8 * c, w);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) u[i][e] *= r * w[e];
+    *reinterpret_cast<uint4*>(out + 8 * c) = pack8(u[i]);
+  }
+}
+
+// How a row of D elements is shared: lanes per row and pieces per lane, or a block of `threads`.
+struct Split {
+  bool block;
+  int v, lanes, threads;
+};
+inline Split split_of(int D) {
+  const int pieces = D / 8;
+  if (pieces <= 128) {
+    int lanes = 8;
+    while (lanes < 32 && lanes < pieces) lanes <<= 1;
+    return Split{false, pieces <= lanes ? 1 : pieces <= 2 * lanes ? 2 : 4, lanes, 256};
+  }
+  int threads = 128;
+  while (threads < 512 && threads * 2 < pieces) threads <<= 1;      // two pieces a thread up to 8192 elements, four beyond
+  return Split{true, pieces <= 2 * threads ? 2 : 4, 0, threads};
+}
+
+}  // namespace norm
+
+// (kernel template of norm with <kBlock, V> resolved from a Split)
+#define FKDA_NORM_PICK(name, s, ...)                                                                                       \
+  ((s).block ? ((s).v == 2 ? norm::name<true, 2, __VA_ARGS__> : norm::name<true, 4, __VA_ARGS__>)                          \
+             : ((s).v == 1 ? norm::name<false, 1, __VA_ARGS__> : (s).v == 2 ? norm::name<false, 2, __VA_ARGS__> : norm::name<false, 4, __VA_ARGS__>))
+
+cudaError_t launch_gated_norm(const GatedNormParams& p, bool weight_fp32, bool silu, bool gate_first, cudaStream_t stream) {
+  if (p.rows == 0) return cudaSuccess;
+  const norm::Split s = norm::split_of(p.D);
+  const int64_t per = s.block ? 1 : s.threads / s.lanes;
+  const dim3 grid(static_cast<unsigned>((p.rows + per - 1) / per));
+  void (*kernel)(GatedNormParams, int);
+  if (weight_fp32) kernel = silu ? (gate_first ? FKDA_NORM_PICK(gated_norm_kernel, s, true, true, true) : FKDA_NORM_PICK(gated_norm_kernel, s, true, true, false))
+                                 : (gate_first ? FKDA_NORM_PICK(gated_norm_kernel, s, true, false, true) : FKDA_NORM_PICK(gated_norm_kernel, s, true, false, false));
+  else kernel = silu ? (gate_first ? FKDA_NORM_PICK(gated_norm_kernel, s, false, true, true) : FKDA_NORM_PICK(gated_norm_kernel, s, false, true, false))
+                     : (gate_first ? FKDA_NORM_PICK(gated_norm_kernel, s, false, false, true) : FKDA_NORM_PICK(gated_norm_kernel, s, false, false, false));
+  return launch_after(kernel, grid, static_cast<unsigned>(s.threads), 0, stream, p, s.lanes);
+}
+
+cudaError_t launch_add_norm(const AddNormParams& p, bool weight_fp32, bool residual_fp32, cudaStream_t stream) {
+  if (p.rows == 0) return cudaSuccess;
+  const norm::Split s = norm::split_of(p.D);
+  const int64_t per = s.block ? 1 : s.threads / s.lanes;
+  const dim3 grid(static_cast<unsigned>((p.rows + per - 1) / per));
+  void (*kernel)(AddNormParams, int) = weight_fp32 ? (residual_fp32 ? FKDA_NORM_PICK(add_norm_kernel, s, true, true) : FKDA_NORM_PICK(add_norm_kernel, s, true, false))
+                                                   : (residual_fp32 ? FKDA_NORM_PICK(add_norm_kernel, s, false, true) : FKDA_NORM_PICK(add_norm_kernel, s, false, false));
+  return launch_after(kernel, grid, static_cast<unsigned>(s.threads), 0, stream, p, s.lanes);
+}
+
+}  // namespace fkda

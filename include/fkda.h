@@ -1,5 +1,6 @@
 /*
- * fkda.h -- C ABI of the B200 (sm_100a) Kimi Delta Attention prefill.
+ * fkda.h -- C ABI of the B200 (sm_100a) Kimi Delta Attention prefill, and of the operators that a layer has round it:
+ * short convolution, selective state space scan, gated and residual norms.
  *
  * This is the drop-in boundary for the reference's one operator, `flash_kda.fwd`.  It replaces
  * the reference's host op `fwd(...)` (csrc/flash_kda.cpp:28-217), its workspace sizing
@@ -167,6 +168,133 @@ int fkda_fwd_static_ws(const fkda_fwd_params* p, void* cuda_stream);
 int64_t fkda_static_ws_capacity(void);
 int fkda_static_ws_read_status(void* cuda_stream, int* status);
 const char* fkda_static_ws_last_error(void);
+
+/* ---- the operators round the recurrence ---------------------------------------------------------------------------
+ * No counterparts in the reference.  The same contract as fkda_fwd: device pointers on the current device, enqueued on the given
+ * stream, nothing allocated, nothing synchronised, argument errors before anything is launched.
+ *
+ * Tensors [B][T][...] may be columns of wider ones: elements of a token are dense, `*_token_stride` and `*_batch_stride` count
+ * elements from token to token and from batch row to batch row (any value where there is only one; rows may not overlap).  bf16 tensors
+ * start on 16 bytes and have strides that are multiples of 8; dt is exempt from both.  With cu_seqlens B is 1, T counts all tokens,
+ * and rows outside [cu_seqlens[0], cu_seqlens[N]) are neither read for a sequence nor written; its values are not read on the host:
+ * sequences that are not monotone inside [0, T] give undefined results inside the tensors' memory.
+ * An output that shares memory with an input is refused unless the operator's own comment allows it. */
+
+/* Depthwise causal convolution of 2 to 4 taps: y[t][c] = act(bias[c] + sum_k weight[c][k] x[t - (width-1) + k][c]), act = SiLU or none.
+ * States [N][width-1][C] bf16 hold a sequence's last inputs, the oldest first; final_state may be initial_state itself. */
+typedef struct fkda_conv_params {
+  const void* x;             /* bf16 [B][T][C], C a multiple of 8 */
+  const void* weight;        /* [C][width] of weight_dtype, dense */
+  const void* bias;          /* [C] of weight_dtype, or NULL */
+  void* out;                 /* bf16 [B][T][C] */
+  const void* initial_state; /* or NULL: zeros */
+  void* final_state;         /* or NULL */
+  const int64_t* cu_seqlens; /* device int64 [N+1], or NULL for B sequences of T tokens */
+  int64_t B;
+  int64_t T;
+  int64_t C;
+  int64_t N;
+  int64_t x_batch_stride;
+  int64_t x_token_stride;
+  int64_t out_batch_stride;
+  int64_t out_token_stride;
+  int32_t width;
+  int32_t weight_dtype;      /* FKDA_STATE_BF16 or FKDA_STATE_FP32 */
+  int32_t silu;              /* 0: no activation */
+} fkda_conv_params;
+int fkda_short_conv(const fkda_conv_params* p, void* cuda_stream);
+
+/* Selective state space scan with one decay per head: with delta = softplus(dt + dt_bias[h]),
+ *   S_t = exp(-exp(A_log[h]) delta) S_(t-1) + delta x_t B_t^T,   out_t = S_t C_t + D[h] x_t
+ * Heads h * G / H share a group's B and C.  P is 64 or 128, Ns (the columns of a state) 64 or 128, H a multiple of G.
+ * A value that is not finite reaches, beside everything after it, the tokens of its own block of 128 from the sequence's start. */
+typedef struct fkda_ssm_params {
+  const void* x;             /* bf16 [B][T][H][P] */
+  const void* dt;            /* bf16 [B][T][H] */
+  const void* Bm;            /* bf16 [B][T][G][Ns] */
+  const void* Cm;            /* bf16 [B][T][G][Ns] */
+  void* out;                 /* bf16 [B][T][H][P] */
+  const float* A_log;        /* fp32 [H] */
+  const float* dt_bias;      /* fp32 [H] */
+  const float* D;            /* fp32 [H], or NULL: no skip connection */
+  const void* initial_state; /* [N][H][P][Ns] of state_dtype, or NULL: zeros */
+  void* final_state;         /* same shape and dtype, or NULL; may be initial_state itself */
+  const int64_t* cu_seqlens; /* device int64 [N+1], or NULL for B sequences of T tokens */
+  void* workspace;           /* >= fkda_ssm_scratch_bytes bytes, 256-byte aligned (NULL where that is 0) */
+  int64_t workspace_bytes;
+  int64_t B;
+  int64_t T;
+  int64_t H;
+  int64_t P;
+  int64_t G;
+  int64_t Ns;
+  int64_t N;                 /* sequences */
+  int64_t x_batch_stride;
+  int64_t x_token_stride;
+  int64_t dt_batch_stride;
+  int64_t dt_token_stride;
+  int64_t B_batch_stride;
+  int64_t B_token_stride;
+  int64_t C_batch_stride;
+  int64_t C_token_stride;
+  int64_t out_batch_stride;
+  int64_t out_token_stride;
+  int32_t state_dtype;       /* fkda_state_dtype of initial_state / final_state */
+} fkda_ssm_params;
+int fkda_ssm_scratch_bytes(const fkda_ssm_params* p, int64_t* bytes);
+int fkda_ssm_fwd(const fkda_ssm_params* p, void* cuda_stream);
+
+/* Root-mean-square norm over the D channels of every (token, head) with a gate a = sigmoid(g) or g sigmoid(g):
+ *   out = x / rms(x) * weight * a,   or with gate_first   out = (x a) / rms(x a) * weight,   rms(u) = sqrt(mean(u^2) + eps)
+ * out may be x or gate itself (same address and strides). */
+typedef struct fkda_gated_norm_params {
+  const void* x;             /* bf16 [B][T][H][D], D a multiple of 8 up to 16384 */
+  const void* gate;          /* bf16 [B][T][H][D] */
+  const void* weight;        /* [D], or [H][D] with weight_per_head, of weight_dtype, dense */
+  void* out;                 /* bf16 [B][T][H][D] */
+  int64_t B;
+  int64_t T;
+  int64_t H;
+  int64_t D;
+  int64_t x_batch_stride;
+  int64_t x_token_stride;
+  int64_t gate_batch_stride;
+  int64_t gate_token_stride;
+  int64_t out_batch_stride;
+  int64_t out_token_stride;
+  float eps;
+  int32_t weight_dtype;
+  int32_t weight_per_head;
+  int32_t silu;              /* 0: a = sigmoid(g) */
+  int32_t gate_first;
+} fkda_gated_norm_params;
+int fkda_gated_norm(const fkda_gated_norm_params* p, void* cuda_stream);
+
+/* h = residual + scale x;  residual_out = h;  out = h / rms(h) * weight, from h before it is rounded to residual_dtype.
+ * residual_out may be residual itself and out may be x itself (same address and strides). */
+typedef struct fkda_add_norm_params {
+  const void* x;             /* bf16 [B][T][D], D a multiple of 8 up to 16384 */
+  const void* residual;      /* [B][T][D] of residual_dtype */
+  const void* weight;        /* [D] of weight_dtype */
+  void* out;                 /* bf16 [B][T][D] */
+  void* residual_out;        /* [B][T][D] of residual_dtype */
+  int64_t B;
+  int64_t T;
+  int64_t D;
+  int64_t x_batch_stride;
+  int64_t x_token_stride;
+  int64_t residual_batch_stride;
+  int64_t residual_token_stride;
+  int64_t out_batch_stride;
+  int64_t out_token_stride;
+  int64_t residual_out_batch_stride;
+  int64_t residual_out_token_stride;
+  float scale;
+  float eps;
+  int32_t weight_dtype;
+  int32_t residual_dtype;
+} fkda_add_norm_params;
+int fkda_add_norm(const fkda_add_norm_params* p, void* cuda_stream);
 
 /* Message of the last error on this thread ("" if none). */
 const char* fkda_last_error(void);
