@@ -37,7 +37,7 @@ class SsmParams(ctypes.Structure):
     """Mirror of `fkda_ssm_params`."""
     _fields_ = (_fields(_P, "x", "dt", "Bm", "Cm", "out", "A_log", "dt_bias", "D", "initial_state", "final_state", "cu_seqlens", "workspace")
                 + _fields(_I64, "workspace_bytes", "B", "T", "H", "P", "G", "Ns", "N") + _rows("x", "dt", "B", "C", "out")
-                + _fields(_I32, "state_dtype"))
+                + _fields(_I32, "state_dtype") + [("flags", ctypes.c_uint32)])
 
 
 class GatedNormParams(ctypes.Structure):
@@ -188,7 +188,7 @@ def _ssm_params(x, dt, Bm, Cm, out, A_log, dt_bias, D, initial_state, final_stat
     return SsmParams(_ptr(x), _ptr(dt), _ptr(Bm), _ptr(Cm), _ptr(out), _ptr(A_log), _ptr(dt_bias), _ptr(D), _ptr(initial_state),
                      _ptr(final_state), _ptr(cu_seqlens), None, 0, batch, T, H, P, G, Ns, N, *_tokens(x, "x", x.shape),
                      *_tokens(dt, "dt", (batch, T, H)), *_tokens(Bm, "B", (batch, T, G, Ns)), *_tokens(Cm, "C", (batch, T, G, Ns)),
-                     *_tokens(out, "out", x.shape), state_dtype)
+                     *_tokens(out, "out", x.shape), state_dtype, 0)
 
 
 def ssm_fwd(x, dt, B, C, out, A_log, dt_bias, D=None, initial_state=None, final_state=None, cu_seqlens=None, *, workspace=None):

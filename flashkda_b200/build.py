@@ -20,8 +20,8 @@ HOST_EXT = os.path.join(HERE, "_fkda_host" + sysconfig.get_config_var("EXT_SUFFI
 HOST_STAMP = os.path.join(OBJ_DIR, "fkda_host.command")
 PUBLIC_HEADER = os.path.join(os.path.dirname(HERE), "include", "fkda.h")
 SOURCES = ["fkda_api.cu", "fkda_prepare.cu", "fkda_prepare_tc.cu", "fkda_scan.cu", "fkda_scan2.cu", "fkda_recur_split.cu", "fkda_recur.cu", "fkda_operands.cu", "fkda_scan_short.cu", "fkda_segscan.cu", "fkda_short16.cu", "fkda_step.cu", "fkda_refmode.cu", "fkda_aux.cu", "fkda_static_ws.cu",
-           "fkda_layer_api.cu", "fkda_conv.cu", "fkda_norm.cu", "fkda_ssm_step.cu"]
-HEADERS = [os.path.join(CSRC, "fkda_common.cuh"), os.path.join(CSRC, "fkda_tma.cuh"), os.path.join(CSRC, "fkda_elem.cuh"), os.path.join(CSRC, "fkda_record.cuh"), os.path.join(CSRC, "fkda_layer.cuh"), PUBLIC_HEADER,
+           "fkda_layer_api.cu", "fkda_conv.cu", "fkda_norm.cu", "fkda_ssm_step.cu", "fkda_ssm_scan.cu"]
+HEADERS = [os.path.join(CSRC, "fkda_common.cuh"), os.path.join(CSRC, "fkda_tma.cuh"), os.path.join(CSRC, "fkda_elem.cuh"), os.path.join(CSRC, "fkda_record.cuh"), os.path.join(CSRC, "fkda_layer.cuh"), os.path.join(CSRC, "fkda_ssm.cuh"), PUBLIC_HEADER,
            os.path.join(os.path.dirname(HERE), "include", "fkda_testing.h")]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "--use_fast_math", "-Xcompiler", "-fPIC", "-Xptxas", "-v"]

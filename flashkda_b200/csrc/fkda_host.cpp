@@ -279,6 +279,7 @@ PyObject* ssm_fwd_fast(PyObject*, PyObject* const* a, Py_ssize_t n) {
   FKDA_STRIDES(p, B, b);
   FKDA_STRIDES(p, C, c);
   FKDA_STRIDES(p, out, out);
+  p.flags = FKDA_FLAG_STATUS_UNREAD;
   return on_device(dev, [&](void* stream) -> PyObject* {
     if (fkda_ssm_scratch_bytes(&p, &p.workspace_bytes) != FKDA_OK) Py_RETURN_FALSE;
     c10::DataPtr ws;                       // (freed when the call returns, as in fwd_fast)

@@ -2,7 +2,9 @@
 #include <cmath>
 
 #include "../../include/fkda.h"
+#include "../../include/fkda_testing.h"
 #include "fkda_layer.cuh"
+#include "fkda_ssm.cuh"
 
 namespace {
 
@@ -123,12 +125,24 @@ bool over(const View& out, const Sizes& s, const void* parameter, int64_t elemen
     if (rc_ != FKDA_OK) return rc_; \
   } while (0)
 
-int check_ssm(const fkda_ssm_params* p) {
-  if (!p) return refuse("params is NULL");
+int check_ssm_sizes(const fkda_ssm_params* p) {
   FKDA_TRY(check_batch(p->B, p->T, p->N, p->cu_seqlens));
   if (p->H <= 0 || p->H > 65535 || p->G <= 0 || p->H % p->G != 0) return refuse("H must lie in [1, 65535] and be a multiple of G");
   if ((p->P != 64 && p->P != 128) || (p->Ns != 64 && p->Ns != 128)) return refuse("P and the columns of a state must be 64 or 128");
-  if (p->N * p->H > 0x3fffffffLL) return refuse("N*H exceeds 2^30-1 chains");
+  if (p->N * p->H > 0x1fffffffLL) return refuse("N*H exceeds 2^29-1 chains");
+  if (p->T > 0x7fff0000LL || (p->N + p->T / fkda::kSsmBlock * (p->cu_seqlens ? 1 : p->N)) * p->H > 0x3fffffffLL) return refuse("too many tokens for one call");
+  return FKDA_OK;
+}
+// whether every sequence goes token by token
+bool by_token(const fkda_ssm_params* p) { return p->T <= fkda::kSsmStepT; }
+fkda::SsmLayout layout_of(const fkda_ssm_params* p) {
+  return fkda::ssm_layout(p->T, p->N, static_cast<int>(p->H), static_cast<int>(p->P), static_cast<int>(p->G), static_cast<int>(p->Ns), p->cu_seqlens != nullptr,
+                          fkda::device_sm_count());
+}
+
+int check_ssm(const fkda_ssm_params* p) {
+  if (!p) return refuse("params is NULL");
+  FKDA_TRY(check_ssm_sizes(p));
   if (!p->A_log || !p->dt_bias) return refuse("A_log and dt_bias must be non-NULL");
   if ((p->initial_state || p->final_state) && !known(p->state_dtype)) return refuse("state_dtype must be bf16 or fp32 when a state tensor is given");
   const Sizes s{p->B, p->T};
@@ -147,6 +161,53 @@ int check_ssm(const fkda_ssm_params* p) {
   for (const View* v : {&x, &dt, &b, &c, &o})
     if (ranges_meet(p->final_state, states, v->base, span(*v, s))) return set_error(FKDA_ERR_INVALID_ARGUMENT, "final_state shares memory with %s", v->name);
   if (ranges_meet(p->initial_state, states, p->out, span(o, s))) return refuse("out shares memory with initial_state");
+  return FKDA_OK;
+}
+
+int do_ssm(const fkda_ssm_params* p, const fkda::SsmAid& aid, void* cuda_stream) {
+  FKDA_TRY(check_ssm(p));
+  const Sizes s{p->B, p->T};
+  fkda::SsmParams q{};
+  q.x = static_cast<const __nv_bfloat16*>(p->x);
+  q.dt = static_cast<const __nv_bfloat16*>(p->dt);
+  q.Bm = static_cast<const __nv_bfloat16*>(p->Bm);
+  q.Cm = static_cast<const __nv_bfloat16*>(p->Cm);
+  q.out = static_cast<__nv_bfloat16*>(p->out);
+  q.A_log = p->A_log;
+  q.dt_bias = p->dt_bias;
+  q.D = p->D;
+  q.initial_state = p->initial_state;
+  q.final_state = p->final_state;
+  q.cu_seqlens = p->cu_seqlens;
+  q.xs = rows_of(View{"x", p->x, 0, 2, p->x_batch_stride, p->x_token_stride}, s);
+  q.dts = rows_of(View{"dt", p->dt, 0, 2, p->dt_batch_stride, p->dt_token_stride}, s);
+  q.bs = rows_of(View{"B", p->Bm, 0, 2, p->B_batch_stride, p->B_token_stride}, s);
+  q.cs = rows_of(View{"C", p->Cm, 0, 2, p->C_batch_stride, p->C_token_stride}, s);
+  q.os = rows_of(View{"out", p->out, 0, 2, p->out_batch_stride, p->out_token_stride}, s);
+  q.T = p->T;
+  q.H = static_cast<int>(p->H);
+  q.P = static_cast<int>(p->P);
+  q.G = static_cast<int>(p->G);
+  q.Ns = static_cast<int>(p->Ns);
+  q.N = static_cast<int>(p->N);
+  q.state_fp32 = p->state_dtype == FKDA_STATE_FP32;
+  cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
+  cudaError_t e;
+  if (by_token(p)) {
+    e = fkda::launch_ssm_step(q, 0, stream);
+    return e == cudaSuccess ? FKDA_OK : cuda_error(e, "selective scan launch");
+  }
+  const fkda::SsmLayout L = layout_of(p);
+  if (!p->workspace || (reinterpret_cast<uintptr_t>(p->workspace) & 255u)) return refuse("workspace must be non-NULL and 256-byte aligned");
+  if (p->workspace_bytes < L.bytes)
+    return set_error(FKDA_ERR_WORKSPACE_TOO_SMALL, "workspace has %lld bytes, %lld needed", (long long)p->workspace_bytes, (long long)L.bytes);
+  e = fkda::launch_ssm_scan(q, L, aid, p->workspace, !(p->flags & FKDA_FLAG_STATUS_UNREAD), stream);
+  if (e != cudaSuccess) return cuda_error(e, "selective scan launch");
+  if (p->cu_seqlens) {
+    // the sequences of a few tokens, decode steps among the prompts
+    e = fkda::launch_ssm_step(q, fkda::kSsmStepT, stream);
+    if (e != cudaSuccess) return cuda_error(e, "selective scan launch");
+  }
   return FKDA_OK;
 }
 
@@ -194,39 +255,17 @@ int fkda_short_conv(const fkda_conv_params* p, void* cuda_stream) {
 
 int fkda_ssm_scratch_bytes(const fkda_ssm_params* p, int64_t* bytes) {
   if (!p || !bytes) return refuse("NULL pointer");
-  *bytes = 0;
+  FKDA_TRY(check_ssm_sizes(p));
+  *bytes = by_token(p) ? 0 : layout_of(p).bytes;
   return FKDA_OK;
 }
 
-int fkda_ssm_fwd(const fkda_ssm_params* p, void* cuda_stream) {
-  FKDA_TRY(check_ssm(p));
-  const Sizes s{p->B, p->T};
-  fkda::SsmParams q{};
-  q.x = static_cast<const __nv_bfloat16*>(p->x);
-  q.dt = static_cast<const __nv_bfloat16*>(p->dt);
-  q.Bm = static_cast<const __nv_bfloat16*>(p->Bm);
-  q.Cm = static_cast<const __nv_bfloat16*>(p->Cm);
-  q.out = static_cast<__nv_bfloat16*>(p->out);
-  q.A_log = p->A_log;
-  q.dt_bias = p->dt_bias;
-  q.D = p->D;
-  q.initial_state = p->initial_state;
-  q.final_state = p->final_state;
-  q.cu_seqlens = p->cu_seqlens;
-  q.xs = rows_of(View{"x", p->x, 0, 2, p->x_batch_stride, p->x_token_stride}, s);
-  q.dts = rows_of(View{"dt", p->dt, 0, 2, p->dt_batch_stride, p->dt_token_stride}, s);
-  q.bs = rows_of(View{"B", p->Bm, 0, 2, p->B_batch_stride, p->B_token_stride}, s);
-  q.cs = rows_of(View{"C", p->Cm, 0, 2, p->C_batch_stride, p->C_token_stride}, s);
-  q.os = rows_of(View{"out", p->out, 0, 2, p->out_batch_stride, p->out_token_stride}, s);
-  q.T = p->T;
-  q.H = static_cast<int>(p->H);
-  q.P = static_cast<int>(p->P);
-  q.G = static_cast<int>(p->G);
-  q.Ns = static_cast<int>(p->Ns);
-  q.N = static_cast<int>(p->N);
-  q.state_fp32 = p->state_dtype == FKDA_STATE_FP32;
-  const cudaError_t e = fkda::launch_ssm_step(q, static_cast<cudaStream_t>(cuda_stream));
-  return e == cudaSuccess ? FKDA_OK : cuda_error(e, "selective scan launch");
+int fkda_ssm_fwd(const fkda_ssm_params* p, void* cuda_stream) { return do_ssm(p, fkda::SsmAid{0, 0}, cuda_stream); }
+
+int fkda_debug_ssm_giveup(const fkda_ssm_params* p, int stop_loads_after, int wait_limit_us, void* cuda_stream) {
+  if (stop_loads_after < 1 || wait_limit_us < 1 || wait_limit_us > 1000000)
+    return refuse("stop_loads_after >= 1 and 1 <= wait_limit_us <= 1000000 required");
+  return do_ssm(p, fkda::SsmAid{wait_limit_us, stop_loads_after}, cuda_stream);
 }
 
 int fkda_gated_norm(const fkda_gated_norm_params* p, void* cuda_stream) {

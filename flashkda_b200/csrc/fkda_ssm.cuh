@@ -1,0 +1,130 @@
+// What the block form of the selective scan (fkda_ssm_scan.cu) and the C ABI share: sizes, plan, workspace.
+#pragma once
+#include <cuda.h>
+
+#include "fkda_layer.cuh"
+
+namespace fkda {
+
+constexpr int kSsmBlock = 128;       // tokens of a block
+// Sequences of at most this many tokens go token by token (fkda_ssm_step.cu).
+constexpr int kSsmStepT = 8;
+constexpr int kSsmPlanMost = 2048;   // packed batches of more sequences keep the given order and are not cut into runs
+// Costs of a batch that is cut into runs, in hundredths of a block's full walk: a block of the first pass (states only), what the passes
+// cost beside their blocks, and the chaining of a run.
+constexpr int kSsmFirstCost = 50, kSsmCutCost = 600, kSsmRunCost = 10;
+
+// A packed batch as the plan kernel leaves it: sequences by rank (longest first), prefix sums over the ranks of their runs, and of the
+// runs of those that are cut into more than one (`cut` of them, the first ranks).
+struct SsmPlan {
+  int run_blocks;
+  int active;                // sequences that are walked in blocks
+  int cut;
+  int pad;
+  __host__ __device__ int* order() { return reinterpret_cast<int*>(this + 1); }
+  __host__ __device__ int* prefix(int N) { return order() + N; }
+  __host__ __device__ int* slot_prefix(int N) { return prefix(N) + N + 1; }
+};
+
+struct SsmMaps {
+  CUtensorMap x, b, c, out;
+};
+
+struct SsmScanParams {
+  const __nv_bfloat16* dt;
+  __nv_bfloat16* out;
+  const float* A_log;
+  const float* dt_bias;
+  const float* D;
+  const void* initial_state;
+  void* final_state;
+  const int64_t* cu_seqlens;
+  SsmPlan* plan;             // packed batches
+  float* slots;              // [slot][128][Ns] states of runs, slot = run * pairs + pair
+  float* decays;             // [slot][2] decay over a run, per head
+  int* status;
+  Rows dts, os;
+  int64_t T;
+  int H, P, G, N;
+  int pairs_per_group, pairs;
+  int runs, run_blocks;      // equal lengths
+  int packed;
+  int state_fp32;
+  int split;                 // x' as two bf16 parts
+  int wait_limit_us;         // test aids, as in ScanParams
+  int stop_loads_after;
+};
+
+// One CTA's walk.
+struct SsmItem {
+  int n, group, head0;
+  bool two;                  // the second head is there
+  bool last;                 // the sequence's last run
+  int slot;                  // state to start from (first pass: to leave), or -1: the caller's
+  int blocks;
+  int64_t b, t0, tokens;
+};
+__device__ __forceinline__ SsmItem ssm_item(const SsmScanParams& p, unsigned index, bool full) {
+  SsmItem it{};
+  const int pair = static_cast<int>(index % static_cast<unsigned>(p.pairs));
+  const int rs = static_cast<int>(index / static_cast<unsigned>(p.pairs));
+  int run, runs, len;
+  int64_t bos = 0, eos = p.T;
+  it.slot = -1;
+  if (p.packed) {
+    SsmPlan* plan = p.plan;
+    // (the runs of the first pass are those of the cut sequences, but each one's last: counted with the slots)
+    const int* prefix = full ? plan->prefix(p.N) : plan->slot_prefix(p.N);
+    const int ranks = full ? plan->active : plan->cut;
+    if (ranks == 0 || rs >= prefix[ranks]) return it;
+    int lo = 0, hi = ranks;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (prefix[mid] <= rs) lo = mid; else hi = mid;
+    }
+    run = rs - prefix[lo];
+    runs = prefix[lo + 1] - prefix[lo];
+    if (!full && run + 1 >= runs) return it;
+    len = plan->run_blocks;
+    it.n = plan->order()[lo];
+    if (runs > 1) it.slot = (plan->slot_prefix(p.N)[lo] + run) * p.pairs + pair;
+    bos = p.cu_seqlens[it.n];
+    eos = p.cu_seqlens[it.n + 1];
+    bos = bos < 0 ? 0 : bos > p.T ? p.T : bos;
+    eos = eos < bos ? bos : eos > p.T ? p.T : eos;
+  } else {
+    const int per = full ? p.runs : p.runs - 1;
+    it.n = rs / per;
+    run = rs - it.n * per;
+    runs = p.runs;
+    len = p.run_blocks;
+    it.b = it.n;
+    if (runs > 1) it.slot = (it.n * runs + run) * p.pairs + pair;
+  }
+  it.last = run == runs - 1;
+  it.t0 = bos + (runs > 1 ? static_cast<int64_t>(run) * len * kSsmBlock : 0);
+  it.tokens = it.last ? eos - it.t0 : static_cast<int64_t>(len) * kSsmBlock;
+  it.blocks = static_cast<int>((it.tokens + kSsmBlock - 1) / kSsmBlock);
+  const int per_pair = p.P == 128 ? 1 : 2, in_group = p.H / p.G;
+  it.group = pair / p.pairs_per_group;
+  const int first = (pair - it.group * p.pairs_per_group) * per_pair;
+  it.head0 = it.group * in_group + first;
+  it.two = per_pair == 2 && first + 1 < in_group;
+  return it;
+}
+
+struct SsmLayout {
+  int pairs_per_group, pairs;
+  int runs, run_blocks;      // equal lengths
+  int least;                 // packed: the shortest runs that may be chosen, 0: sequences stay whole
+  int64_t items, first_items, chained, slots;
+  int64_t plan_off, decay_off, slot_off, bytes;
+};
+SsmLayout ssm_layout(int64_t T, int64_t N, int H, int P, int G, int Ns, bool packed, int sms);
+
+struct SsmAid {
+  int wait_limit_us, stop_loads_after;
+};
+cudaError_t launch_ssm_scan(const SsmParams& p, const SsmLayout& L, const SsmAid& aid, void* workspace, bool clear_status, cudaStream_t stream);
+
+}  // namespace fkda

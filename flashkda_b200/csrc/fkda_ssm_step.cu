@@ -22,7 +22,7 @@ constexpr int kThreads = 128;
 __device__ __forceinline__ float softplus(float x) { return fmaxf(x, 0.f) + log1pf(ex2f(-kLog2e * fabsf(x))); }
 
 template <int kNs, bool kFp32, bool kPacked>
-__global__ void __launch_bounds__(kThreads) ssm_step_kernel(const SsmParams p) {
+__global__ void __launch_bounds__(kThreads) ssm_step_kernel(const SsmParams p, int most) {
   constexpr int kLanes = kNs / 8, kRows = 4 * (32 / kLanes) * (kThreads / 32);
   grid_dependency_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, j = lane % kLanes;
@@ -37,6 +37,7 @@ __global__ void __launch_bounds__(kThreads) ssm_step_kernel(const SsmParams p) {
     bos = bos < 0 ? 0 : bos > p.T ? p.T : bos;
     eos = eos < bos ? bos : eos > p.T ? p.T : eos;
     len = eos - bos;
+    if (most > 0 && len > most) return;
     b = 0;
   }
   const int64_t state = (static_cast<int64_t>(chain) * p.P + row) * kNs + 4 * j;
@@ -129,17 +130,17 @@ __global__ void __launch_bounds__(kThreads) ssm_step_kernel(const SsmParams p) {
 }
 
 template <int kNs>
-cudaError_t launch(const SsmParams& p, cudaStream_t stream) {
+cudaError_t launch(const SsmParams& p, int most, cudaStream_t stream) {
   const int64_t blocks = static_cast<int64_t>(p.N) * p.H * (p.P / (kNs == 128 ? 32 : 64));
   auto kernel = p.cu_seqlens != nullptr ? (p.state_fp32 ? ssm_step_kernel<kNs, true, true> : ssm_step_kernel<kNs, false, true>)
                                         : (p.state_fp32 ? ssm_step_kernel<kNs, true, false> : ssm_step_kernel<kNs, false, false>);
-  return launch_after(kernel, dim3(static_cast<unsigned>(blocks)), kThreads, 0, stream, p);
+  return launch_after(kernel, dim3(static_cast<unsigned>(blocks)), kThreads, 0, stream, p, most);
 }
 
 }  // namespace ssm_step
 
-cudaError_t launch_ssm_step(const SsmParams& p, cudaStream_t stream) {
-  return p.Ns == 128 ? ssm_step::launch<128>(p, stream) : ssm_step::launch<64>(p, stream);
+cudaError_t launch_ssm_step(const SsmParams& p, int most, cudaStream_t stream) {
+  return p.Ns == 128 ? ssm_step::launch<128>(p, most, stream) : ssm_step::launch<64>(p, most, stream);
 }
 
 }  // namespace fkda

@@ -36,6 +36,11 @@ int fkda_debug_plan_slice(int64_t chains, int64_t chunks_per_sequence);
  * Nothing is in flight when the wait runs out.  Read the outcome with fkda_read_status. */
 int fkda_debug_scan_giveup(const fkda_fwd_params* p, int stop_copies_after, int wait_limit_us, void* cuda_stream);
 
+/* The give-up path of the selective scan over blocks: fkda_ssm_fwd in which no CTA loads more than `stop_loads_after` blocks of its walk
+ * and every wait gives up after `wait_limit_us` microseconds.  A longer walk then finds a barrier that nothing will complete; its CTA must
+ * record status 2, release its tensor memory and return. */
+int fkda_debug_ssm_giveup(const fkda_ssm_params* p, int stop_loads_after, int wait_limit_us, void* cuda_stream);
+
 /* The same for the token-parallel stage: fkda_prepare on the pipelined kernel, in which every CTA loads the tiles of
  * its first item only and every wait gives up after `wait_limit_us` microseconds.  A CTA with a second item waits for
  * tiles that nothing will bring; it must record status 2, wait for what it still has in flight, release its tensor
