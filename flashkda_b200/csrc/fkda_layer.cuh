@@ -92,4 +92,17 @@ __device__ __forceinline__ void load8(const void* base, int64_t at, float (&w)[8
 // 1 / (1 + e^-x) to fp32 accuracy (the tanh approximation has an absolute error that small values do not bear)
 __device__ __forceinline__ float sigmoid_exact(float x) { return __fdividef(1.f, 1.f + ex2f(-kLog2e * x)); }
 
+// max(x, 0) + log(1 + e^-|x|) to fp32 accuracy.  log(1 + u) = 2 atanh(z) with z = u / (2 + u) <= 1/3, by the series of atanh to z^13: what is
+// left out is below 2^-26 of the sum.
+__device__ __forceinline__ float softplus(float x) {
+  const float u = ex2f(-kLog2e * fabsf(x)), z = __fdividef(u, 2.f + u), q = z * z;
+  float s = fmaf(q, 1.f / 13.f, 1.f / 11.f);
+  s = fmaf(q, s, 1.f / 9.f);
+  s = fmaf(q, s, 1.f / 7.f);
+  s = fmaf(q, s, 1.f / 5.f);
+  s = fmaf(q, s, 1.f / 3.f);
+  s = fmaf(q, s, 1.f);
+  return fmaf(2.f * z, s, fmaxf(x, 0.f));
+}
+
 }  // namespace fkda

@@ -203,11 +203,6 @@ int do_ssm(const fkda_ssm_params* p, const fkda::SsmAid& aid, void* cuda_stream)
     return set_error(FKDA_ERR_WORKSPACE_TOO_SMALL, "workspace has %lld bytes, %lld needed", (long long)p->workspace_bytes, (long long)L.bytes);
   e = fkda::launch_ssm_scan(q, L, aid, p->workspace, !(p->flags & FKDA_FLAG_STATUS_UNREAD), stream);
   if (e != cudaSuccess) return cuda_error(e, "selective scan launch");
-  if (p->cu_seqlens) {
-    // the sequences of a few tokens, decode steps among the prompts
-    e = fkda::launch_ssm_step(q, fkda::kSsmStepT, stream);
-    if (e != cudaSuccess) return cuda_error(e, "selective scan launch");
-  }
   return FKDA_OK;
 }
 

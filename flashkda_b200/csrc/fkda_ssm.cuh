@@ -10,9 +10,9 @@ constexpr int kSsmBlock = 128;       // tokens of a block
 // Sequences of at most this many tokens go token by token (fkda_ssm_step.cu).
 constexpr int kSsmStepT = 8;
 constexpr int kSsmPlanMost = 2048;   // packed batches of more sequences keep the given order and are not cut into runs
-// Costs of a batch that is cut into runs, in hundredths of a block's full walk: a block of the first pass (states only), what the passes
-// cost beside their blocks, and the chaining of a run.
-constexpr int kSsmFirstCost = 50, kSsmCutCost = 600, kSsmRunCost = 10;
+// What the planner of runs reckons with, in hundredths of a block's walk (some 3 us): a block of the first pass, what a walk takes beside its
+// blocks, the launch that chains runs, and (in hundredths of that) what a run's state of a pair of heads takes on its way through memory.
+constexpr int kSsmFirstCost = 48, kSsmStartCost = 170, kSsmChainCost = 150, kSsmSlotCost = 175;
 
 // A packed batch as the plan kernel leaves it: sequences by rank (longest first), prefix sums over the ranks of their runs, and of the
 // runs of those that are cut into more than one (`cut` of them, the first ranks).
@@ -20,7 +20,8 @@ struct SsmPlan {
   int run_blocks;
   int active;                // sequences that are walked in blocks
   int cut;
-  int pad;
+  unsigned next[2];          // walks handed out so far: first pass, second pass
+  int pad[3];
   __host__ __device__ int* order() { return reinterpret_cast<int*>(this + 1); }
   __host__ __device__ int* prefix(int N) { return order() + N; }
   __host__ __device__ int* slot_prefix(int N) { return prefix(N) + N + 1; }
@@ -43,6 +44,7 @@ struct SsmScanParams {
   float* slots;              // [slot][128][Ns] states of runs, slot = run * pairs + pair
   float* decays;             // [slot][2] decay over a run, per head
   int* status;
+  unsigned* queue;           // packed batches: counter that hands the walks out, or nullptr: a CTA each
   Rows dts, os;
   int64_t T;
   int H, P, G, N;
@@ -50,13 +52,13 @@ struct SsmScanParams {
   int runs, run_blocks;      // equal lengths
   int packed;
   int state_fp32;
-  int split;                 // x' as two bf16 parts
   int wait_limit_us;         // test aids, as in ScanParams
   int stop_loads_after;
 };
 
 // One CTA's walk.
 struct SsmItem {
+  bool there;                // false: no more walks
   int n, group, head0;
   bool two;                  // the second head is there
   bool last;                 // the sequence's last run
@@ -71,12 +73,14 @@ __device__ __forceinline__ SsmItem ssm_item(const SsmScanParams& p, unsigned ind
   int run, runs, len;
   int64_t bos = 0, eos = p.T;
   it.slot = -1;
+  it.there = !p.packed;
   if (p.packed) {
     SsmPlan* plan = p.plan;
     // (the runs of the first pass are those of the cut sequences, but each one's last: counted with the slots)
     const int* prefix = full ? plan->prefix(p.N) : plan->slot_prefix(p.N);
     const int ranks = full ? plan->active : plan->cut;
     if (ranks == 0 || rs >= prefix[ranks]) return it;
+    it.there = true;
     int lo = 0, hi = ranks;
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;

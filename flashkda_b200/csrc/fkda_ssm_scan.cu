@@ -5,16 +5,19 @@
 //     G = C B^T,   M_ij = G_ij 2^(l_i - l_j) delta_j  (j <= i),   out = M X + 2^(l_i) (C S^T) + D X
 //     S <- 2^(l_127) S + X'^T B,   x'_j = 2^(l_127 - l_j) delta_j x_j
 // A CTA walks the blocks of 128 rows of a sequence's states: two heads of P = 64 that share B and C, or one of P = 128.  Five products a block,
-// 128 x 128 x 128 each (two of them X'^T B): G, Z = C S^T, X' as hi + lo (below), Y = M X.  Nineteen warps:
-//     0-7    M from G, in tensor memory over G itself (rows i = lanes; the even warpgroup takes the column blocks 0 and 2, the odd one 1 and 3), then
-//            out = Y + 2^l Z + D x over the tile of x in shared memory, from where a tensor copy takes it
-//     8-11   the state: fp32 in tensor memory, once a block read, rescaled and written back, and its bf16 copy for Z
-//     12-15  delta and the decays of the next block; x' in steps of 16 tokens
-//     16     loads of B and C       17     products       18     loads of x, stores of out
+// 128 x 128 x 128 each: G, C S^T, X'^T B twice (X' as hi + lo, below), M X.  Tensor memory holds G and over it M; the output, first as C S^T,
+// then rescaled by rows, then with M X on top; X'^T; and S.  Twenty warps:
+//     0-15   M from G: a warp a 32 x 32 block (rows i = lanes)
+//     0-7    the output's rescaling (rows i = lanes, half of the columns each warpgroup); then out = that + D x over the tile of x in shared
+//            memory, from where a tensor copy takes it
+//     8-15   the state: fp32 in tensor memory, once a block read, rescaled and written back, and its bf16 copy for C S^T (half the columns
+//            each warpgroup); then X'^T (half the rows each), by transposing ldmatrix, whose fragments are those of tcgen05.st
+//     16, 18 delta and the decays, a head each       17     products       19     tensor copies (beside the rows of M with the most to do)
 //
-// Roundings: G, Y, Z and S accumulate in fp32.  M and the state's copy for Z are bf16 operands, as out is bf16.  The state is what a
-// caller keeps, so X' goes into its product as hi + lo, two bf16 parts that hold 16 bits, where the state is asked for in fp32; where it is
-// asked for in bf16, or not at all, as one.
+// Roundings: all products accumulate in fp32.  M and the state's copy are bf16 operands, as out is bf16.  The state is what a
+// caller keeps, so X' goes into its product as hi + lo, two bf16 parts that hold 16 bits.  They come straight from x, which is bf16, and the
+// token's weight as wh + wl: hi = round(x wh), whose error x wh - hi is a bf16 number itself, and lo = round((x wh - hi) + x wl): three
+// instructions for two elements, where unpacking, an fp32 product and two conversions took eight.
 // Decays: every exponent that is evaluated is a sum of terms of one sign, so that nothing cancels, but for those within 32 x 32 blocks on
 // the diagonal, which are differences of sums over less than 32 tokens.
 // Rows past a sequence's end are zeroed in the tiles of x and B where they are summed over; those of C only reach outputs that are not stored.
@@ -27,45 +30,66 @@ namespace fkda {
 namespace ssm_scan {
 
 constexpr int kQ = kSsmBlock;
-constexpr int kThreads = 19 * 32;
-constexpr int kSlots = 3;                        // steps of x' under way
-constexpr int kSlotBytes = 2 * 16 * 128 * 2;     // hi | lo, each [2 halves of 64 columns][16 tokens][128 B]
+constexpr int kThreads = 20 * 32;          // (registers are given to four warps at a time: a twenty-first would leave 80 a thread)
 constexpr int kTileX = kQ * 128 * 2;
-constexpr uint32_t kColG = 0, kColY = 128, kColZ = 256, kColS = 384;     // tensor memory; M lies over G
+constexpr int kXs = 3;                           // tiles of x: one being read, one with its output on the way out, one on the way in
+constexpr int kScals = 4;                        // blocks whose decays are at hand: they are worked out ahead
+constexpr uint32_t kColG = 0, kColY = 128, kColX = 256 /* hi, then lo */, kColS = 384;     // tensor memory; M lies over G
 
-// Per block and head, written by warps 12-15.
+// Per block and head, written by warps 16 and 18.
 struct Scalars {
   float p[2][kQ];          // running sum of a from the start of the token's 32-token block, itself included
-  float lp[2][kQ];         // p - log2(delta)
+  float g[2][kQ];          // delta 2^-p; where the block's sum is beyond kMostDecay instead p - log2(delta)
   float f[2][kQ];          // delta 2^(sum of a behind the token to the end of its 32-token block)
-  float w[2][kQ];          // ... to the end of the block of 128
+  uint2 w[2][kQ / 2];      // f decayed to the end of the block of 128, two tokens a word: as bf16, and what that leaves as bf16
   float tot[2][4];         // sums over the four 32-token blocks
   float decay[2];          // 2^(sum over all)
   float pad[6];
 };
 
+// Decay within a 32-token block up to which 2^(p_i - p_j) is taken as 2^p_i 2^-p_j: both factors, and delta with them, stay normal numbers.
+constexpr float kMostDecay = -100.f;
+// Masks of a 32 x 32 triangle for pairs of bf16: row i, 16 words, rows 80 bytes apart (16-byte reads of eight rows then meet no bank twice).
+constexpr int kMaskPitch = 80;
+
 template <int kNs>
 struct Smem {
   static constexpr int kTile = kQ * kNs * 2;
-  static constexpr int kB = 0, kC = kB + 2 * kTile, kX = kC + kTile, kS = kX + 2 * kTileX, kXp = kS + 128 * kNs * 2;
-  static constexpr int kScal = kXp + kSlots * kSlotBytes, kBars = kScal + 2 * static_cast<int>(sizeof(Scalars)), kMisc = kBars + 256;
-  static constexpr int kBytes = kMisc + 64;
+  static constexpr int kB = 0, kC = kB + kTile, kX = kC + kTile, kS = kX + kXs * kTileX;
+  static constexpr int kScal = kS + 128 * kNs * 2, kBars = kScal + kScals * static_cast<int>(sizeof(Scalars)), kMisc = kBars + 256;
+  static constexpr int kMask = kMisc + 64, kBytes = kMask + 32 * kMaskPitch;
 };
 static_assert(Smem<128>::kBytes <= 227 * 1024, "shared memory of a CTA");
 
 enum {
-  B_FULL_B = 0 /*[2]*/, B_EMPTY_B = 2 /*[2]*/, B_FULL_C = 4, B_EMPTY_C, B_FULL_X /*[2]*/, B_EMPTY_X = 8 /*[2]*/, B_XP_FULL = 10 /*[kSlots]*/, B_XP_EMPTY = 13 /*[kSlots]*/,
-  B_SCAL = 16 /*[2]*/, B_SCAL_FREE = 18 /*[2]*/, B_G = 20, B_M, B_Y, B_ZY_FREE, B_S_FULL, B_S_READY, B_OUT /*[2]*/, B_DRAIN = 28, B_MEET, B_COUNT
+  B_FULL_B = 0, B_FULL_C, B_Z /* C S^T done, C free */, B_FULL_X /*[kXs]*/, B_EMPTY_X = 6 /*[kXs]*/, B_OUT = 9 /*[kXs]*/, B_XT = 12 /*[2]*/, B_SCAL = 14 /*[kScals]*/,
+  B_SCAL_FREE = 18 /*[kScals]*/, B_G = 22, B_Y, B_M, B_Y_FREE, B_S_FULL /* X'^T B done, B free */, B_S_READY, B_DRAIN, B_MEET, B_COUNT,
+  B_EMPTY_B = B_G, B_XT2 = B_OUT      // of the first pass, [2] each: buffer c & 1 of B and X'^T free; X'^T of the second buffer
 };
 static_assert(B_COUNT * 8 <= 256, "barrier area");
+
+// Arrivals that complete a phase of barrier `i`.
+template <bool kFull, bool kWide>
+__device__ __forceinline__ uint32_t arrivals(int i) {
+  if (i >= B_SCAL && i < B_SCAL + kScals) return kWide ? 1 : 2;
+  if (i >= B_EMPTY_X && i < B_XT + 2) return 8;                       // (EMPTY_X, OUT, XT)
+  if (i >= B_SCAL_FREE && i < B_SCAL_FREE + kScals) return kFull ? 16 : 8;
+  if (i == B_M) return 16;
+  return i == B_Y_FREE || i == B_S_READY || i == B_MEET ? 8 : 1;
+}
+__device__ __forceinline__ void mbar_inval(uint32_t bar) { asm volatile("mbarrier.inval.shared::cta.b64 [%0];" ::"r"(bar) : "memory"); }
 
 // Shared-memory matrix descriptor of a tile with the 128-byte swizzle (rows of 128 bytes, 1024-byte aligned groups of eight).  K-major: `sbo`
 // is the distance between groups of eight rows (M or N), 16 elements along K are 32 bytes on.  MN-major (rows along K): `sbo` is the
 // distance between groups of eight rows along K, `lbo` between blocks of 64 elements of M or N.
 __device__ __forceinline__ uint64_t desc_sw128(uint32_t addr, uint32_t lbo) { return umma_desc(addr, lbo, 1024) | (2ull << 61); }
 
+// (What follows a first attempt is kept out of line: a sub-partition's instruction cache holds some 500 instructions, which four roles share.)
+__device__ __noinline__ bool wait_on(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
+}
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
-  return __all_sync(0xffffffffu, mbar_wait_parked(bar, parity, abort_flag));
+  return __all_sync(0xffffffffu, mbar_try_wait(bar, parity)) || wait_on(bar, parity, abort_flag);
 }
 __device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
@@ -81,8 +105,17 @@ __device__ __forceinline__ void drain(uint32_t bar, uint32_t parity) {
   while (!mbar_test(bar, parity) && globaltimer_ns() - t0 < 20000000ull) {
   }
 }
-// 2^-|x| is at most 1, so neither branch overflows.
-__device__ __forceinline__ float softplus(float x) { return fmaxf(x, 0.f) + log1pf(ex2f(-kLog2e * fabsf(x))); }
+// Products of bf16 pairs, rounded to bf16.
+__device__ __forceinline__ uint32_t mul_bf2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t fma_bf2(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
 using elem::f2;
 using elem::fma2;
 using elem::mul;
@@ -90,6 +123,62 @@ using elem::pk;
 using elem::upk;
 __device__ __forceinline__ f2 pk(uint32_t a, uint32_t b) { return elem::pk(__uint_as_float(a), __uint_as_float(b)); }
 __device__ __forceinline__ uint32_t round2(f2 x) { return elem::round_bf(x); }
+
+// (clears what lies above the diagonal, whatever it is: row `mask` of the table)
+__device__ __forceinline__ void keep_triangle(uint32_t (&m)[16], const uint8_t* mask) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint4 k = *reinterpret_cast<const uint4*>(mask + 16 * j);
+    m[4 * j] &= k.x;
+    m[4 * j + 1] &= k.y;
+    m[4 * j + 2] &= k.z;
+    m[4 * j + 3] &= k.w;
+  }
+}
+
+// M of the 32 x 32 block (w, b) from G, over it: 16 columns a head.  (One copy for all sixteen warps that make M: see wait_on.)
+template <bool kWide>
+__device__ __noinline__ void make_m(uint32_t at, const Scalars& s, int b, int w, const uint8_t* masks) {
+  const int lane = threadIdx.x & 31;
+  uint32_t g[32];
+  at += 32 * b;
+  if (b > w) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) g[i] = 0u;
+    tmem_st32(at, g);
+    return;
+  }
+  tmem_ld32(at, g);
+  tmem_wait_ld();
+#pragma unroll 1
+  for (int h = 0; h < (kWide ? 1 : 2); ++h) {
+    uint32_t m[16];
+    const float4 tot = *reinterpret_cast<const float4*>(s.tot[h]);
+    // (with the sums over the 32-token blocks between the two)
+    const float r = s.p[h][32 * w + lane] + (b < 1 && w > 1 ? tot.y : 0.f) + (b < 2 && w > 2 ? tot.z : 0.f);
+    if (b < w || (w == 0 ? tot.x : w == 1 ? tot.y : w == 2 ? tot.z : tot.w) >= kMostDecay) {
+      const float e = ex2f(r);
+      const f2 r2 = pk(e, e);
+      const float4* f = reinterpret_cast<const float4*>((b < w ? s.f[h] : s.g[h]) + 32 * b);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float4 v = f[j];
+        m[2 * j] = round2(mul(pk(g[4 * j], g[4 * j + 1]), mul(r2, pk(v.x, v.y))));
+        m[2 * j + 1] = round2(mul(pk(g[4 * j + 2], g[4 * j + 3]), mul(r2, pk(v.z, v.w))));
+      }
+    } else {
+      // (differences of exponents that have to be taken before the power)
+      const float2* lp = reinterpret_cast<const float2*>(s.g[h] + 32 * b);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const float2 v = lp[j];
+        m[j] = pack_bf16(__uint_as_float(g[2 * j]) * ex2f(r - v.x), __uint_as_float(g[2 * j + 1]) * ex2f(r - v.y));
+      }
+    }
+    if (b == w) keep_triangle(m, masks + lane * kMaskPitch);
+    tmem_st16(at + 16 * h, m);
+  }
+}
 
 // kWide: one head of P = 128, else two of P = 64.  kFull: the outputs too, else only what a run adds to a zero state.
 template <int kNs, bool kWide, bool kFull>
@@ -103,202 +192,183 @@ __global__ void __launch_bounds__(kThreads, 1) ssm_scan_kernel(const __grid_cons
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kMisc + 4);
   Scalars* scal = reinterpret_cast<Scalars*>(smem + L::kScal);
 
-  if (tid == 0) {
-    // the swizzled tiles need this alignment: report instead of computing garbage (below zero: a wait limit, test aid)
-    *abort_flag = (sbase & 1023u) != 0u ? 1 : -p.wait_limit_us;
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(bar(B_FULL_B + i), 1);
-      mbar_init(bar(B_EMPTY_B + i), 1);
-      mbar_init(bar(B_FULL_X + i), 1);
-      mbar_init(bar(B_EMPTY_X + i), 4);
-      mbar_init(bar(B_SCAL + i), 4);
-      mbar_init(bar(B_SCAL_FREE + i), 8);
-      mbar_init(bar(B_OUT + i), 8);
-    }
-    for (int i = 0; i < kSlots; ++i) {
-      mbar_init(bar(B_XP_FULL + i), 4);
-      mbar_init(bar(B_XP_EMPTY + i), 1);
-    }
-    mbar_init(bar(B_FULL_C), 1);
-    mbar_init(bar(B_EMPTY_C), 1);
-    mbar_init(bar(B_G), 1);
-    mbar_init(bar(B_M), 8);
-    mbar_init(bar(B_Y), 1);
-    mbar_init(bar(B_ZY_FREE), 8);
-    mbar_init(bar(B_S_FULL), 1);
-    mbar_init(bar(B_S_READY), 4);
-    mbar_init(bar(B_DRAIN), 1);
-    mbar_init(bar(B_MEET), 4);
-    fence_mbar_init();
+  if (tid < 4) prefetch_tensormap(&maps.x + tid);
+  // the swizzled tiles need this alignment: report instead of computing garbage (below zero: a wait limit, test aid)
+  if (tid == 0) *abort_flag = (sbase & 1023u) != 0u ? 1 : -p.wait_limit_us;
+  if (kFull && tid < 512) {
+    const int i = tid >> 4, j = 2 * (tid & 15);
+    *reinterpret_cast<uint32_t*>(smem + L::kMask + i * kMaskPitch + 2 * j) = (j <= i ? 0xffffu : 0u) | (j + 1 <= i ? 0xffff0000u : 0u);
   }
   if (warp == 17) {
     tmem_alloc(smem_u32(tmem_slot), 512);
     tmem_relinquish();
   }
+  uint32_t tmem_base = 0;
+  volatile unsigned* next = reinterpret_cast<volatile unsigned*>(smem + L::kMisc + 8);
+  grid_dependency_wait();
+  // Packed batches: as many CTAs as there are SMs take one walk after the other, the longest first.
+  for (unsigned turn = 0;; ++turn) {
+  if (warp == 0) {
+    if (lane == 0) *next = p.queue != nullptr ? atomicAdd(p.queue, 1u) : blockIdx.x;
+    if (lane < B_COUNT) {
+      if (turn > 0) mbar_inval(bar(lane));
+      mbar_init(bar(lane), arrivals<kFull, kWide>(lane));
+    }
+    fence_mbar_init();
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+  tmem_base = tmem;
   bool ok = *abort_flag <= 0;
-  grid_dependency_wait();
-  const SsmItem it = ssm_item(p, blockIdx.x, kFull);
+  const SsmItem it = ssm_item(p, *next, kFull);
   const int blocks = ok ? it.blocks : 0;
-
   if (warp < 8) {
     if constexpr (kFull) {
       const int q = warp >> 2, w = warp & 3;                          // column blocks q, q + 2; rows 32 w + lane
       const uint32_t lanes = tmem + (static_cast<uint32_t>(32 * w) << 16);
-      const int head = it.head0 + (kWide ? 0 : q);
-      const bool mine = kWide || q == 0 || it.two;
-      const float D = p.D != nullptr && mine ? __ldg(p.D + head) : 0.f;
+      const bool mine = kWide || q == 0 || it.two;                    // (this warpgroup's half of the output)
+      const float D = blocks > 0 && mine && p.D != nullptr ? __ldg(p.D + it.head0 + (kWide ? 0 : q)) : 0.f;
       for (int c = 0; c < blocks; ++c) {
-        const Scalars& s = scal[c & 1];
-        if (!(ok = warp_wait(bar(B_SCAL + (c & 1)), (c >> 1) & 1, abort_flag))) break;
+        const Scalars& s = scal[c % kScals];
+        if (!(ok = warp_wait(bar(B_SCAL + c % kScals), (c / kScals) & 1, abort_flag))) break;
         if (!(ok = warp_wait(bar(B_G), c & 1, abort_flag))) break;
         tc_fence_after();
-        float pi[2];
-#pragma unroll
-        for (int h = 0; h < (kWide ? 1 : 2); ++h) pi[h] = s.p[h][32 * w + lane];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const int b = q + 2 * k;
-          if (b > w) {
-            uint32_t zero[32];
-#pragma unroll
-            for (int i = 0; i < 32; ++i) zero[i] = 0u;
-            tmem_st32(lanes + kColG + 32 * b, zero);
-            continue;
-          }
-          uint32_t g[32];
-          tmem_ld32(lanes + kColG + 32 * b, g);
-          tmem_wait_ld();
-#pragma unroll
-          for (int h = 0; h < (kWide ? 1 : 2); ++h) {
-            uint32_t m[16];
-            if (b < w) {
-              float between = 0.f;                                    // (sums over the 32-token blocks between the two)
-              if (b < 1 && w > 1) between += s.tot[h][1];
-              if (b < 2 && w > 2) between += s.tot[h][2];
-              const float r = ex2f(pi[h] + between);
-              const f2 r2 = pk(r, r);
-              const float4* f = reinterpret_cast<const float4*>(s.f[h] + 32 * b);
-#pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                const float4 v = f[j];
-                m[2 * j] = round2(mul(pk(g[4 * j], g[4 * j + 1]), mul(r2, pk(v.x, v.y))));
-                m[2 * j + 1] = round2(mul(pk(g[4 * j + 2], g[4 * j + 3]), mul(r2, pk(v.z, v.w))));
-              }
-            } else {
-              const float4* lp = reinterpret_cast<const float4*>(s.lp[h] + 32 * b);
-#pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                const float4 v = lp[j];
-                const float e0 = 4 * j <= lane ? __uint_as_float(g[4 * j]) * ex2f(pi[h] - v.x) : 0.f;
-                const float e1 = 4 * j + 1 <= lane ? __uint_as_float(g[4 * j + 1]) * ex2f(pi[h] - v.y) : 0.f;
-                const float e2 = 4 * j + 2 <= lane ? __uint_as_float(g[4 * j + 2]) * ex2f(pi[h] - v.z) : 0.f;
-                const float e3 = 4 * j + 3 <= lane ? __uint_as_float(g[4 * j + 3]) * ex2f(pi[h] - v.w) : 0.f;
-                m[2 * j] = pack_bf16(e0, e1);
-                m[2 * j + 1] = pack_bf16(e2, e3);
-              }
-            }
-            tmem_st16(lanes + kColG + 32 * b + 16 * h, m);
-          }
-        }
+        make_m<kWide>(lanes + kColG, s, q, w, smem + L::kMask);
         const int hq = kWide ? 0 : q;
         float before = 0.f;
-        for (int k = 0; k < w; ++k) before += s.tot[hq][k];
-        const float e = ex2f(pi[hq] + before);
+        if (w > 0) before += s.tot[hq][0];
+        if (w > 1) before += s.tot[hq][1];
+        if (w > 2) before += s.tot[hq][2];
+        const float e = ex2f(s.p[hq][32 * w + lane] + before);
+        // C S^T -> what the rows' decays leave of it
+        if (!(ok = warp_wait(bar(B_Z), c & 1, abort_flag))) break;
+        tc_fence_after();
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {
+          uint32_t y[32];
+          tmem_ld32(lanes + kColY + 64 * q + 32 * half, y);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) mul2(y[2 * i], y[2 * i + 1], make_float2(e, e));
+          tmem_st32(lanes + kColY + 64 * q + 32 * half, y);
+        }
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) {
           mbar_arrive(bar(B_M));
-          mbar_arrive(bar(B_SCAL_FREE + (c & 1)));
+          mbar_arrive(bar(B_SCAL_FREE + c % kScals));
         }
-
+        // ---- out ----------------------------------------------------------------------------------------------------------------
         if (!(ok = warp_wait(bar(B_Y), c & 1, abort_flag))) break;
         tc_fence_after();
         const int row = 32 * w + lane;
-        const uint32_t xrow = sbase + L::kX + (c & 1) * kTileX + q * (kTileX / 2) + row * 128;
-        const f2 e2 = pk(e, e), D2 = pk(D, D);
-#pragma unroll
+        const uint32_t xrow = sbase + L::kX + (c % kXs) * kTileX + q * (kTileX / 2) + row * 128;
+        const f2 D2 = pk(D, D);
+#pragma unroll 1
         for (int half = 0; half < 2; ++half) {
-          uint32_t y[32], z[32];
+          uint32_t y[32];
+          uint4 x[4];
           tmem_ld32(lanes + kColY + 64 * q + 32 * half, y);
-          tmem_ld32(lanes + kColZ + 64 * q + 32 * half, z);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[j] = lds128(xrow + (((4 * half + j) ^ (row & 7)) << 4));
           tmem_wait_ld();
           if (half == 1) {
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(bar(B_ZY_FREE));
+            if (lane == 0) mbar_arrive(bar(B_Y_FREE));
           }
-          if (!mine) continue;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const uint32_t at = xrow + (((4 * half + j) ^ (row & 7)) << 4);
-            f2 v[4];
+            const uint32_t xv[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
+            uint32_t o[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = fma2(pk(z[8 * j + 2 * i], z[8 * j + 2 * i + 1]), e2, pk(y[8 * j + 2 * i], y[8 * j + 2 * i + 1]));
-            if (p.D != nullptr) {
-              const uint4 xv = lds128(at);
-              v[0] = fma2(pk(bf_lo(xv.x), bf_hi(xv.x)), D2, v[0]);
-              v[1] = fma2(pk(bf_lo(xv.y), bf_hi(xv.y)), D2, v[1]);
-              v[2] = fma2(pk(bf_lo(xv.z), bf_hi(xv.z)), D2, v[2]);
-              v[3] = fma2(pk(bf_lo(xv.w), bf_hi(xv.w)), D2, v[3]);
-            }
-            sts128(at, round2(v[0]), round2(v[1]), round2(v[2]), round2(v[3]));
+            for (int i = 0; i < 4; ++i) o[i] = round2(fma2(pk(bf_lo(xv[i]), bf_hi(xv[i])), D2, pk(y[8 * j + 2 * i], y[8 * j + 2 * i + 1])));
+            if (mine) sts128(xrow + (((4 * half + j) ^ (row & 7)) << 4), o[0], o[1], o[2], o[3]);
           }
         }
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar(B_OUT + (c & 1)));
+        if (lane == 0) mbar_arrive(bar(B_OUT + c % kXs));
       }
     }
-  } else if (warp < 12) {
-    // ---- the state: this thread's row of 128 --------------------------------------------------------------------------------
-    const int row = 32 * (warp & 3) + lane, h = kWide ? 0 : row >> 6;
-    const uint32_t at = tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16) + kColS;
+  } else if (warp < 16) {
+    // ---- the state (this thread's row of 128, half of its columns), then x' (every other step) -----------------------------------
+    const int g = (warp - 8) >> 2, row = 32 * (warp & 3) + lane, h = kWide ? 0 : row >> 6;
+    constexpr int kOwn = kNs / 2;                                     // columns g * kOwn ..
+    const uint32_t at = tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16) + kColS + g * kOwn;
     const bool there = kWide || h == 0 || it.two;
-    const int64_t state = (static_cast<int64_t>(it.n) * p.H + it.head0 + h) * (kWide ? 128 : 64) * kNs + static_cast<int64_t>(kWide ? row : row & 63) * kNs;
-    const uint32_t srow = sbase + L::kS + row * 128;
-    // (32 columns of the state before a block -> its copy for Z; rescaled to the block's end)
-    auto copy_out = [&](const uint32_t (&v)[32], int part) {
+    const int64_t state = ((static_cast<int64_t>(it.n) * p.H + it.head0 + h) * (kWide ? 128 : 64) + (kWide ? row : row & 63)) * kNs + g * kOwn;
+    float* slot = it.slot >= 0 ? p.slots + (static_cast<int64_t>(it.slot) * 128 + row) * kNs + g * kOwn : nullptr;
+    const int t = tid - 8 * 32;
+    // X'^T: this warp's 16 rows of 32, 64 tokens at a time.  A transposed 8 x 8 tile of x has two tokens of a channel in a register, as
+    // tensor memory wants them (register 2j | 2j + 1: lane t/4 | t/4 + 8, column 4j + t%4).
+    auto weigh = [&](uint32_t x, const Scalars& s, uint32_t column, int done) {
+      const uint32_t src = x + ((warp & 3) >> 1) * (kTileX / 2) + (8 * (lane >> 4) + (lane & 7)) * 128 + (((4 * (warp & 1) + 2 * g + ((lane >> 3) & 1)) ^ (lane & 7)) << 4);
+      const uint32_t xt = tmem + (static_cast<uint32_t>(32 * (warp & 3) + 16 * g) << 16) + column;
+#pragma unroll 1
+      for (int th = 0; th < 2; ++th) {
+        uint32_t hi[16], lo[16];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        sts128(srow + (part >> 1) * 16384 + (((4 * (part & 1) + j) ^ (row & 7)) << 4), pack_bf16(__uint_as_float(v[8 * j]), __uint_as_float(v[8 * j + 1])),
-               pack_bf16(__uint_as_float(v[8 * j + 2]), __uint_as_float(v[8 * j + 3])), pack_bf16(__uint_as_float(v[8 * j + 4]), __uint_as_float(v[8 * j + 5])),
-               pack_bf16(__uint_as_float(v[8 * j + 6]), __uint_as_float(v[8 * j + 7])));
-    };
-    auto rescale = [&](uint32_t (&v)[32], float d) {
+        for (int j = 0; j < 8; j += 2) ldsm_x4_trans(src + (64 * th + 8 * j) * 128, hi[2 * j], hi[2 * j + 1], hi[2 * j + 2], hi[2 * j + 3]);
+        const uint2* w = s.w[kWide ? 0 : h] + 32 * th + (lane & 3);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) mul2(v[2 * i], v[2 * i + 1], make_float2(d, d));
+        for (int j = 0; j < 8; ++j) {
+          const uint2 wj = w[4 * j];
+#pragma unroll
+          for (int i = 2 * j; i < 2 * j + 2; ++i) {
+            const uint32_t xi = hi[i];
+            hi[i] = mul_bf2(xi, wj.x);
+            lo[i] = fma_bf2(xi, wj.y, fma_bf2(xi, wj.x, hi[i] ^ 0x80008000u));
+          }
+        }
+        tmem_st_16x128b_x8(xt + 32 * th, hi);
+        tmem_st_16x128b_x8(xt + 64 + 32 * th, lo);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(done + th));
+      }
     };
-    const float* slot = it.slot >= 0 ? p.slots + (static_cast<int64_t>(it.slot) * 128 + row) * kNs : nullptr;
-    for (int c = 0; blocks > 0 && c <= blocks; ++c) {
-      if (c > 0) {
-        if (!(ok = warp_wait(bar(B_S_FULL), (c - 1) & 1, abort_flag))) break;
+    if constexpr (!kFull) {
+      // First pass: from the run's last block to its first, with weights that decay to the run's end, so that nothing is ever rescaled.
+      // Two buffers of X'^T (the second one where G would be) and of B.
+      for (int c = 0; c < blocks; ++c) {
+        if (!(ok = warp_wait(bar(B_SCAL + c % kScals), (c / kScals) & 1, abort_flag))) break;
+        if (!(ok = warp_wait(bar(B_FULL_X + c % kXs), (c / kXs) & 1, abort_flag))) break;
+        if (c >= 2) {
+          if (!(ok = warp_wait(bar(B_EMPTY_B + (c & 1)), ((c >> 1) - 1) & 1, abort_flag))) break;
+          tc_fence_after();
+        }
+        weigh(sbase + L::kX + (c % kXs) * kTileX, scal[c % kScals], c & 1 ? kColG : kColX, c & 1 ? B_XT2 : B_XT);
+        if (lane == 0) {
+          mbar_arrive(bar(B_SCAL_FREE + c % kScals));
+          mbar_arrive(bar(B_EMPTY_X + c % kXs));
+        }
+      }
+      if (ok && blocks > 0 && (ok = warp_wait(bar(B_S_FULL), 0, abort_flag))) {
         tc_fence_after();
-      }
-      float d = 1.f;
-      if (c < blocks) {
-        if (!(ok = warp_wait(bar(B_SCAL + (c & 1)), (c >> 1) & 1, abort_flag))) break;
-        d = scal[c & 1].decay[h];
-      }
-#pragma unroll
-      for (int part = 0; part < kNs / 32; ++part) {
-        uint32_t v[32];
-        if (c > 0) {
+#pragma unroll 1
+        for (int part = 0; part < kOwn / 32; ++part) {
+          uint32_t v[32];
           tmem_ld32(at + 32 * part, v);
           tmem_wait_ld();
-        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(slot + 32 * part + 4 * i) = *reinterpret_cast<const uint4*>(v + 4 * i);
+        }
+      }
+    } else {
+      if (blocks > 0) {
+#pragma unroll 1
+        for (int part = 0; part < kOwn / 32; ++part) {
+          uint32_t v[32];
 #pragma unroll
           for (int i = 0; i < 32; ++i) v[i] = 0u;
-          if (kFull && there) {
-            if (slot != nullptr) {
-#pragma unroll
-              for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(v + 4 * i) = *reinterpret_cast<const uint4*>(slot + 32 * part + 4 * i);
-            } else if (p.initial_state != nullptr && p.state_fp32) {
-              const float* src = static_cast<const float*>(p.initial_state) + state + 32 * part;
+          if (there) {
+            if (slot != nullptr || (p.initial_state != nullptr && p.state_fp32)) {
+              const float* src = (slot != nullptr ? slot : static_cast<const float*>(p.initial_state) + state) + 32 * part;
 #pragma unroll
               for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(v + 4 * i) = *reinterpret_cast<const uint4*>(src + 4 * i);
             } else if (p.initial_state != nullptr) {
@@ -315,16 +385,43 @@ __global__ void __launch_bounds__(kThreads, 1) ssm_scan_kernel(const __grid_cons
               }
             }
           }
-        }
-        if (c < blocks) {
-          if constexpr (kFull) copy_out(v, part);
-          rescale(v, d);
           tmem_st32(at + 32 * part, v);
-        } else if (there) {
-          if (!kFull) {
+        }
+        tmem_wait_st();
+      }
+      for (int c = 0; blocks > 0 && c <= blocks; ++c) {
+        float d = 1.f;
+        if (c > 0) {
+          if (!(ok = warp_wait(bar(B_S_FULL), (c - 1) & 1, abort_flag))) break;
+          tc_fence_after();
+        }
+        const Scalars& s = scal[c % kScals];
+        if (c < blocks) {
+          if (!(ok = warp_wait(bar(B_SCAL + c % kScals), (c / kScals) & 1, abort_flag))) break;
+          d = s.decay[h];
+        }
+#pragma unroll 1
+        for (int part = 0; part < kOwn / 32; ++part) {
+          uint32_t v[32];
+          tmem_ld32(at + 32 * part, v);
+          tmem_wait_ld();
+          uint32_t word[16];                                            // as bf16
 #pragma unroll
-            for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(const_cast<float*>(slot) + 32 * part + 4 * i) = *reinterpret_cast<const uint4*>(v + 4 * i);
-          } else if (it.last && p.final_state != nullptr) {
+          for (int i = 0; i < 16; ++i) word[i] = pack_bf16(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+          if (c < blocks) {
+            if constexpr (kFull) {
+              // the copy for C S^T (that of the block before has been read: its product came before those of the state)
+              const uint32_t dst = sbase + L::kS + row * 128;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int piece = g * (kOwn / 8) + 4 * part + i;
+                sts128(dst + (piece >> 3) * 16384 + (((piece & 7) ^ (row & 7)) << 4), word[4 * i], word[4 * i + 1], word[4 * i + 2], word[4 * i + 3]);
+              }
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mul2(v[2 * i], v[2 * i + 1], make_float2(d, d));
+            tmem_st32(at + 32 * part, v);
+          } else if (there && it.last && p.final_state != nullptr) {
             if (p.state_fp32) {
               float* dst = static_cast<float*>(p.final_state) + state + 32 * part;
 #pragma unroll
@@ -332,254 +429,239 @@ __global__ void __launch_bounds__(kThreads, 1) ssm_scan_kernel(const __grid_cons
             } else {
               __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.final_state) + state + 32 * part;
 #pragma unroll
-              for (int i = 0; i < 4; ++i)
-                *reinterpret_cast<uint4*>(dst + 8 * i) =
-                    make_uint4(pack_bf16(__uint_as_float(v[8 * i]), __uint_as_float(v[8 * i + 1])), pack_bf16(__uint_as_float(v[8 * i + 2]), __uint_as_float(v[8 * i + 3])),
-                               pack_bf16(__uint_as_float(v[8 * i + 4]), __uint_as_float(v[8 * i + 5])), pack_bf16(__uint_as_float(v[8 * i + 6]), __uint_as_float(v[8 * i + 7])));
+              for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(dst + 8 * i) = make_uint4(word[4 * i], word[4 * i + 1], word[4 * i + 2], word[4 * i + 3]);
             }
           }
         }
-      }
-      if (c < blocks) {
-        tmem_wait_st();
-        tc_fence_before();
-        if constexpr (kFull) fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(B_S_READY));
-      }
-    }
-  } else if (warp < 16) {
-    // ---- decays, and x' ------------------------------------------------------------------------------------------------------
-    const int t = tid - 12 * 32, v = warp - 12;
-    const int heads[2] = {it.head0, it.head0 + (!kWide && it.two ? 1 : 0)};
-    float A[2], bias[2];
-    if (blocks > 0) {
-#pragma unroll
-      for (int h = 0; h < (kWide ? 1 : 2); ++h) {
-        A[h] = -kLog2e * ex2f(kLog2e * __ldg(p.A_log + heads[h]));
-        bias[h] = __ldg(p.dt_bias + heads[h]);
-      }
-    }
-    float dt[2] = {0.f, 0.f};
-    auto load_dt = [&](int c) {
-      if (c >= blocks || static_cast<int64_t>(c) * kQ + t >= it.tokens) return;
-      const __nv_bfloat16* src = p.dt + it.b * p.dts.batch + (it.t0 + static_cast<int64_t>(c) * kQ + t) * p.dts.token;
-#pragma unroll
-      for (int h = 0; h < (kWide ? 1 : 2); ++h) dt[h] = __bfloat162float(src[heads[h]]);
-    };
-    // (a rendezvous of these four warps whose wait is bounded, too)
-    uint32_t meetings = 0;
-    auto meet = [&] {
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(B_MEET));
-      return warp_wait(bar(B_MEET), meetings++ & 1, abort_flag);
-    };
-    float log_decay[2] = {0.f, 0.f};                                 // of the blocks so far (thread 0)
-    auto scalars = [&](int c) {
-      if (c >= blocks) return true;
-      Scalars& s = scal[c & 1];
-      if (kFull && c >= 2 && !warp_wait(bar(B_SCAL_FREE + (c & 1)), ((c >> 1) - 1) & 1, abort_flag)) return false;
-      const bool valid = static_cast<int64_t>(c) * kQ + t < it.tokens;
-      float f[2], tot[2];
-#pragma unroll
-      for (int h = 0; h < (kWide ? 1 : 2); ++h) {
-        const float delta = valid ? softplus(dt[h] + bias[h]) : 0.f;
-        const float a = valid ? A[h] * delta : 0.f;
-        float up = a, down = __shfl_down_sync(0xffffffffu, a, 1);
-        if (lane == 31) down = 0.f;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-          const float u = __shfl_up_sync(0xffffffffu, up, d), e = __shfl_down_sync(0xffffffffu, down, d);
-          if (lane >= d) up += u;
-          if (lane + d < 32) down += e;
-        }
-        f[h] = delta * ex2f(down);
-        tot[h] = __shfl_sync(0xffffffffu, up, 31);
-        s.p[h][t] = up;
-        s.lp[h][t] = up - __log2f(delta);
-        s.f[h][t] = f[h];
-        if (lane == 0) s.tot[h][v] = tot[h];
-      }
-      load_dt(c + 1);
-      if (!meet()) return false;
-#pragma unroll
-      for (int h = 0; h < (kWide ? 1 : 2); ++h) {
-        const float4 all = *reinterpret_cast<const float4*>(s.tot[h]);
-        const float behind = (v < 1 ? all.y : 0.f) + (v < 2 ? all.z : 0.f) + (v < 3 ? all.w : 0.f), sum = (all.x + all.y) + (all.z + all.w);
-        s.w[h][t] = f[h] * ex2f(behind);
-        if (t == 0) s.decay[h] = ex2f(sum);
-        log_decay[h] += sum;
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(B_SCAL + (c & 1)));
-      return meet();                                                  // (w of all tokens, for x')
-    };
-    load_dt(0);
-    if (blocks > 0) ok = scalars(0);
-    uint32_t step = 0;
-    const int tok = t >> 3, chunk = t & 7;
-    for (int c = 0; ok && c < blocks; ++c) {
-      if (!(ok = scalars(c + 1))) break;
-      const Scalars& s = scal[c & 1];
-      if (!(ok = warp_wait(bar(B_FULL_X + (c & 1)), (c >> 1) & 1, abort_flag))) break;
-      const uint32_t x = sbase + L::kX + (c & 1) * kTileX;
-      const int64_t left = it.tokens - static_cast<int64_t>(c) * kQ;
-      if (left < kQ) {
-        if (!(ok = warp_wait(bar(B_FULL_B + (c & 1)), (c >> 1) & 1, abort_flag))) break;
-        const uint32_t b = sbase + L::kB + (c & 1) * L::kTile;
-        for (int i = t; i < (kQ - static_cast<int>(left)) * 8; i += 128) {
-          const uint32_t off = (static_cast<uint32_t>(left) + i / 8) * 128 + (i % 8) * 16;
-          sts128(x + off, 0u, 0u, 0u, 0u);
-          sts128(x + kTileX / 2 + off, 0u, 0u, 0u, 0u);
-          sts128(b + off, 0u, 0u, 0u, 0u);
-          if (kNs == 128) sts128(b + L::kTile / 2 + off, 0u, 0u, 0u, 0u);
-        }
-        fence_proxy_async_smem();
-        if (!(ok = meet())) break;
-      }
-      for (int st = 0; st < 8; ++st, ++step) {
-        const uint32_t sl = step % kSlots, use = step / kSlots;
-        if (use > 0 && !(ok = warp_wait(bar(B_XP_EMPTY + sl), (use - 1) & 1, abort_flag))) break;
-        const int tt = 16 * st + tok;
-        const uint32_t dst = sbase + L::kXp + sl * kSlotBytes + tok * 128 + ((chunk ^ (tok & 7)) << 4);
-        const uint32_t src = x + tt * 128 + ((chunk ^ (tt & 7)) << 4);
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const float w = s.w[kWide ? 0 : half][tt];
-          const uint4 xv = lds128(src + half * (kTileX / 2));
-          const uint32_t in[4] = {xv.x, xv.y, xv.z, xv.w};
-          const f2 w2 = pk(w, w);
-          uint32_t hi[4], lo[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const f2 y = mul(pk(bf_lo(in[i]), bf_hi(in[i])), w2);
-            hi[i] = round2(y);
-            const f2 rest = fma2(pk(bf_lo(hi[i]), bf_hi(hi[i])), pk(-1.f, -1.f), y);
-            lo[i] = round2(rest);
+        if (c < blocks) {
+          tmem_wait_st();
+          tc_fence_before();
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(B_S_READY));
+
+          if (!(ok = warp_wait(bar(B_FULL_X + c % kXs), (c / kXs) & 1, abort_flag))) break;
+          const uint32_t x = sbase + L::kX + (c % kXs) * kTileX;
+          const int64_t left = it.tokens - static_cast<int64_t>(c) * kQ;
+          if (kFull && left < kQ) {
+            // the last block: rows past the end, in the tiles whose rows are summed over
+            if (!(ok = warp_wait(bar(B_FULL_B), c & 1, abort_flag))) break;
+            const uint32_t b = sbase + L::kB;
+            for (int i = t; i < (kQ - static_cast<int>(left)) * 8; i += 256) {
+              const uint32_t off = (static_cast<uint32_t>(left) + i / 8) * 128 + (i % 8) * 16;
+              sts128(x + off, 0u, 0u, 0u, 0u);
+              sts128(x + kTileX / 2 + off, 0u, 0u, 0u, 0u);
+              sts128(b + off, 0u, 0u, 0u, 0u);
+              if (kNs == 128) sts128(b + L::kTile / 2 + off, 0u, 0u, 0u, 0u);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(B_MEET));
+            if (!(ok = warp_wait(bar(B_MEET), 0, abort_flag))) break;
           }
-          sts128(dst + half * 2048, hi[0], hi[1], hi[2], hi[3]);
-          if (p.split) sts128(dst + kSlotBytes / 2 + half * 2048, lo[0], lo[1], lo[2], lo[3]);
+          weigh(x, s, kColX, B_XT);
+          if constexpr (kFull) {
+            if (!(ok = warp_wait(bar(B_G), c & 1, abort_flag))) break;
+            tc_fence_after();
+            make_m<kWide>(tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16) + kColG, s, 2 + g, warp & 3, smem + L::kMask);
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+          }
+          if (lane == 0) {
+            mbar_arrive(bar(B_SCAL_FREE + c % kScals));
+            mbar_arrive(bar(B_M));
+          }
         }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(B_XP_FULL + sl));
       }
-      if (!ok) break;
-      if (!kFull) {
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(B_EMPTY_X + (c & 1)));
-      }
-    }
-    if (!kFull && ok && t == 0 && blocks > 0) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) p.decays[2 * it.slot + h] = ex2f(log_decay[kWide ? 0 : h]);
-    }
-  } else if (warp == 16) {
-    // ---- loads of B and C ------------------------------------------------------------------------------------------------------
-    int issued = 0;
-    const int column = it.group * kNs;
-    for (int c = 0; c < blocks && c < p.stop_loads_after; ++c) {
-      const int buf = c & 1, row = static_cast<int>(it.t0) + c * kQ;
-      if (c >= 2 && !(ok = warp_wait(bar(B_EMPTY_B + buf), ((c >> 1) - 1) & 1, abort_flag))) break;
-      if (lane == 0) {
-        mbar_arrive_expect_tx(bar(B_FULL_B + buf), L::kTile);
-#pragma unroll
-        for (int i = 0; i < kNs / 64; ++i) tma_load_3d(sbase + L::kB + buf * L::kTile + i * 16384, &maps.b, column + 64 * i, row, static_cast<int>(it.b), bar(B_FULL_B + buf));
-      }
-      issued = c + 1;
-      if constexpr (kFull) {
-        if (c >= 1 && !(ok = warp_wait(bar(B_EMPTY_C), (c - 1) & 1, abort_flag))) break;
-        if (lane == 0) {
-          mbar_arrive_expect_tx(bar(B_FULL_C), L::kTile);
-#pragma unroll
-          for (int i = 0; i < kNs / 64; ++i) tma_load_3d(sbase + L::kC + i * 16384, &maps.c, column + 64 * i, row, static_cast<int>(it.b), bar(B_FULL_C));
-        }
-        __syncwarp();
-      }
-    }
-    // every copy has landed before this CTA's memory goes to another: those that nobody waited for
-    if (lane == 0) {
-      for (int c = issued > 2 ? issued - 2 : 0; c < issued; ++c) drain(bar(B_FULL_B + (c & 1)), (c >> 1) & 1);
-      if (kFull && issued > 0 && ok) drain(bar(B_FULL_C), (issued - 1) & 1);
-      if (kFull && issued > 1 && !ok) drain(bar(B_FULL_C), (issued - 2) & 1);
     }
   } else if (warp == 17) {
     // ---- products ----------------------------------------------------------------------------------------------------------------
-    constexpr uint32_t idesc_g = umma_idesc_bf16(128, 128, 0, 0), idesc_s = umma_idesc_bf16(128, kNs, 1, 1), idesc_y = umma_idesc_bf16(128, kWide ? 128 : 64, 0, 1);
-    const uint64_t dc = desc_sw128(sbase + L::kC, 16), ds = desc_sw128(sbase + L::kS, 16);
-    uint32_t step = 0;
-    for (int c = 0; c < blocks; ++c) {
-      const int buf = c & 1;
-      const uint32_t b = sbase + L::kB + buf * L::kTile, x = sbase + L::kX + buf * kTileX;
-      if (!(ok = warp_wait(bar(B_FULL_B + buf), (c >> 1) & 1, abort_flag))) break;
-      if constexpr (kFull) {
-        if (!(ok = warp_wait(bar(B_FULL_C), c & 1, abort_flag))) break;
-        if (c > 0 && !(ok = warp_wait(bar(B_Y), (c - 1) & 1, abort_flag))) break;       // M of the block before has been read
-        tc_fence_after();
-        if (elect_one()) {
-          const uint64_t db = desc_sw128(b, 16);
+    constexpr uint32_t idesc_g = umma_idesc_bf16(128, 128, 0, 0), idesc_s = umma_idesc_bf16(128, kNs, 0, 1), idesc_y = umma_idesc_bf16(128, kWide ? 128 : 64, 0, 1);
+    // S += X'^T B over 64 tokens: hi, then lo
+    auto add_state = [&](uint32_t b, uint32_t xt, int th, bool onto) {
+      const uint64_t db = desc_sw128(b + th * 8192, 16384);
 #pragma unroll
-          for (int k = 0; k < kNs / 16; ++k) umma_ss(tmem + kColG, dc + (k / 4) * 1024 + (k % 4) * 2, db + (k / 4) * 1024 + (k % 4) * 2, idesc_g, k > 0);
-          umma_commit(bar(B_G));
-        }
-        __syncwarp();
+      for (int k = 0; k < 4; ++k) {
+        umma_ts(tmem + kColS, tmem + xt + 32 * th + 8 * k, db + k * 128, idesc_s, onto || k > 0);
+        umma_ts(tmem + kColS, tmem + xt + 64 + 32 * th + 8 * k, db + k * 128, idesc_s, 1);
       }
-      if (!(ok = warp_wait(bar(B_S_READY), c & 1, abort_flag))) break;
-      if constexpr (kFull) {
-        if (c > 0 && !(ok = warp_wait(bar(B_ZY_FREE), (c - 1) & 1, abort_flag))) break;
-        tc_fence_after();
-        if (elect_one()) {
-#pragma unroll
-          for (int k = 0; k < kNs / 16; ++k) umma_ss(tmem + kColZ, dc + (k / 4) * 1024 + (k % 4) * 2, ds + (k / 4) * 1024 + (k % 4) * 2, idesc_g, k > 0);
-          umma_commit(bar(B_EMPTY_C));
-        }
-        __syncwarp();
-      }
-      for (int st = 0; st < 8; ++st, ++step) {
-        const uint32_t sl = step % kSlots, use = step / kSlots;
-        if (!(ok = warp_wait(bar(B_XP_FULL + sl), use & 1, abort_flag))) break;
-        tc_fence_after();
-        if (elect_one()) {
-          const uint64_t da = desc_sw128(sbase + L::kXp + sl * kSlotBytes, 2048), db = desc_sw128(b + st * 2048, 16384);
-          umma_ss(tmem + kColS, da, db, idesc_s, 1);
-          if (p.split) umma_ss(tmem + kColS, da + kSlotBytes / 2 / 16, db, idesc_s, 1);
-          umma_commit(bar(B_XP_EMPTY + sl));
-          if (st == 7) {
-            umma_commit(bar(B_EMPTY_B + buf));
-            umma_commit(bar(B_S_FULL));
+    };
+    if constexpr (!kFull) {
+      for (int c = 0; c < blocks; ++c) {
+        if (!(ok = warp_wait(bar(B_FULL_B + (c & 1)), (c >> 1) & 1, abort_flag))) break;
+        for (int th = 0; th < 2; ++th) {
+          if (!(ok = warp_wait(bar((c & 1 ? B_XT2 : B_XT) + th), (c >> 1) & 1, abort_flag))) break;
+          tc_fence_after();
+          if (elect_one()) {
+            add_state(sbase + L::kB + (c & 1) * L::kTile, c & 1 ? kColG : kColX, th, c + th > 0);
+            if (th == 1) {
+              if (c + 2 < blocks) umma_commit(bar(B_EMPTY_B + (c & 1)));
+              else if (c + 1 == blocks) umma_commit(bar(B_S_FULL));
+            }
           }
+          __syncwarp();
+        }
+        if (!ok) break;
+      }
+    }
+    const uint64_t dc = desc_sw128(sbase + L::kC, 16), ds = desc_sw128(sbase + L::kS, 16);
+    for (int c = 0; kFull && c < blocks; ++c) {
+      const uint32_t b = sbase + L::kB, x = sbase + L::kX + (c % kXs) * kTileX;
+      if (!(ok = warp_wait(bar(B_FULL_B), c & 1, abort_flag))) break;
+      if (!(ok = warp_wait(bar(B_FULL_C), c & 1, abort_flag))) break;
+      if (c > 0 && !(ok = warp_wait(bar(B_Y), (c - 1) & 1, abort_flag))) break;       // M of the block before has been read
+      tc_fence_after();
+      if (elect_one()) {
+        const uint64_t db = desc_sw128(b, 16);
+#pragma unroll
+        for (int k = 0; k < kNs / 16; ++k) umma_ss(tmem + kColG, dc + (k / 4) * 1024 + (k % 4) * 2, db + (k / 4) * 1024 + (k % 4) * 2, idesc_g, k > 0);
+        umma_commit(bar(B_G));
+      }
+      __syncwarp();
+      if (!(ok = warp_wait(bar(B_S_READY), c & 1, abort_flag))) break;
+      if (c > 0 && !(ok = warp_wait(bar(B_Y_FREE), (c - 1) & 1, abort_flag))) break;
+      tc_fence_after();
+      if (elect_one()) {
+#pragma unroll
+        for (int k = 0; k < kNs / 16; ++k) umma_ss(tmem + kColY, dc + (k / 4) * 1024 + (k % 4) * 2, ds + (k / 4) * 1024 + (k % 4) * 2, idesc_g, k > 0);
+        umma_commit(bar(B_Z));
+      }
+      __syncwarp();
+      for (int th = 0; th < 2; ++th) {
+        if (!(ok = warp_wait(bar(B_XT + th), c & 1, abort_flag))) break;
+        tc_fence_after();
+        if (elect_one()) {
+          add_state(b, kColX, th, true);
+          if (th == 1) umma_commit(bar(B_S_FULL));
         }
         __syncwarp();
       }
       if (!ok) break;
-      if constexpr (kFull) {
-        if (!(ok = warp_wait(bar(B_FULL_X + buf), (c >> 1) & 1, abort_flag))) break;
-        if (!(ok = warp_wait(bar(B_M), c & 1, abort_flag))) break;
-        tc_fence_after();
-        if (elect_one()) {
+      if (!(ok = warp_wait(bar(B_FULL_X + c % kXs), (c / kXs) & 1, abort_flag))) break;
+      if (!(ok = warp_wait(bar(B_M), c & 1, abort_flag))) break;
+      tc_fence_after();
+      if (elect_one()) {
 #pragma unroll
-          for (int h = 0; h < (kWide ? 1 : 2); ++h) {
-            const uint64_t dx = desc_sw128(x + h * (kTileX / 2), 16384);
+        for (int h = 0; h < (kWide ? 1 : 2); ++h) {
+          const uint64_t dx = desc_sw128(x + h * (kTileX / 2), 16384);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) umma_ts(tmem + kColY + 64 * h, tmem + kColG + 32 * (k / 2) + 16 * h + 8 * (k % 2), dx + k * 128, idesc_y, k > 0);
-          }
-          umma_commit(bar(B_Y));
+          for (int k = 0; k < 8; ++k) umma_ts(tmem + kColY + 64 * h, tmem + kColG + 32 * (k / 2) + 16 * h + 8 * (k % 2), dx + k * 128, idesc_y, 1);
         }
-        __syncwarp();
+        umma_commit(bar(B_Y));
       }
+      __syncwarp();
     }
     // no product may be under way when the tensor memory is given back
     if (elect_one()) umma_commit(bar(B_DRAIN));
     __syncwarp();
     if (lane == 0) drain(bar(B_DRAIN), 0);
     __syncwarp();
+  } else if (warp != 19) {
+    // ---- delta and the decays of a head: four tokens a lane, eight lanes a 32-token block (the second head's on warp 18) ------------
+    const int h = warp == 16 ? 0 : 1, head = it.head0 + (h == 1 && it.two ? 1 : 0), mine = kWide && h == 1 ? 0 : blocks;
+    float log_decay = 0.f, A = 0.f, bias = 0.f;
+    // dt of this block and the next two: asked for two blocks ahead, as nothing else hides the way to memory
+    const int64_t pitch = p.dts.token, turn_on = (kFull ? kQ : -kQ) * pitch;
+    const int64_t start = kFull || blocks == 0 ? 0 : static_cast<int64_t>(blocks - 1) * kQ;       // (the first pass goes backwards)
+    const unsigned short* src = reinterpret_cast<const unsigned short*>(p.dt) + it.b * p.dts.batch + (it.t0 + start + 4 * lane) * pitch + head;
+    auto load_dt = [&](int c, uint32_t (&to)[4]) {
+      const int64_t left = c < mine ? it.tokens - static_cast<int64_t>(kFull ? c : blocks - 1 - c) * kQ - 4 * lane : 0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) to[k] = k < left ? static_cast<uint32_t>(__ldg(src + k * pitch)) << 16 : 0u;
+      src += turn_on;
+    };
+    uint32_t raw[4], then[4], after_then[4];
+    load_dt(0, raw);
+    load_dt(1, then);
+    if (mine > 0) {
+      A = -kLog2e * ex2f(kLog2e * __ldg(p.A_log + head));
+      bias = __ldg(p.dt_bias + head);
+    }
+#pragma unroll 1
+    for (int c = 0; c < mine; ++c) {
+      Scalars& s = scal[c % kScals];
+      load_dt(c + 2, after_then);
+      const int64_t left = it.tokens - static_cast<int64_t>(kFull ? c : blocks - 1 - c) * kQ - 4 * lane;      // this lane's tokens that are there
+      float d[4], a[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        d[k] = k < left ? softplus(__uint_as_float(raw[k]) + bias) : 0.f;
+        a[k] = k < left ? A * d[k] : 0.f;
+        raw[k] = then[k];
+        then[k] = after_then[k];
+      }
+      const float own = (a[0] + a[1]) + (a[2] + a[3]);
+      float up = own, down = own;                                     // inclusive sums over the eight lanes, forwards and backwards
+#pragma unroll
+      for (int i = 1; i < 8; i <<= 1) {
+        const float u = __shfl_up_sync(0xffffffffu, up, i), e = __shfl_down_sync(0xffffffffu, down, i);
+        if ((lane & 7) >= i) up += u;
+        if ((lane & 7) + i < 8) down += e;
+      }
+      const float before = __shfl_up_sync(0xffffffffu, up, 1), after = __shfl_down_sync(0xffffffffu, down, 1);
+      const float head_sum = (lane & 7) == 0 ? 0.f : before, rest = (lane & 7) == 7 ? 0.f : after;
+      const float t0 = __shfl_sync(0xffffffffu, up, 7), t1 = __shfl_sync(0xffffffffu, up, 15), t2 = __shfl_sync(0xffffffffu, up, 23), t3 = __shfl_sync(0xffffffffu, up, 31);
+      const int block = lane >> 3;
+      const float behind = (block < 1 ? t1 : 0.f) + (block < 2 ? t2 : 0.f) + (block < 3 ? t3 : 0.f);
+      const float sum = (t0 + t1) + (t2 + t3), to_end = ex2f(kFull ? behind : behind + log_decay);
+      log_decay += sum;
+      const float s2 = rest + a[3], s1 = s2 + a[2], s0 = s1 + a[1];
+      const float4 f = make_float4(d[0] * ex2f(s0), d[1] * ex2f(s1), d[2] * ex2f(s2), d[3] * ex2f(rest));
+      const float w0 = f.x * to_end, w1 = f.y * to_end, w2 = f.z * to_end, w3 = f.w * to_end;
+      const uint32_t h01 = pack_bf16(w0, w1), h23 = pack_bf16(w2, w3);
+      const uint4 w = make_uint4(h01, pack_bf16(w0 - bf_lo(h01), w1 - bf_hi(h01)), h23, pack_bf16(w2 - bf_lo(h23), w3 - bf_hi(h23)));
+      if (c >= kScals && !(ok = warp_wait(bar(B_SCAL_FREE + c % kScals), (c / kScals - 1) & 1, abort_flag))) break;
+      reinterpret_cast<uint4*>(s.w[h])[lane] = w;
+      if constexpr (kFull) {
+        const float whole = block == 0 ? t0 : block == 1 ? t1 : block == 2 ? t2 : t3;
+        const float p0 = head_sum + a[0], p1 = p0 + a[1], p2 = p1 + a[2], p3 = p2 + a[3];
+        reinterpret_cast<float4*>(s.p[h])[lane] = make_float4(p0, p1, p2, p3);
+        reinterpret_cast<float4*>(s.g[h])[lane] = whole >= kMostDecay ? make_float4(d[0] * ex2f(-p0), d[1] * ex2f(-p1), d[2] * ex2f(-p2), d[3] * ex2f(-p3))
+                                                                      : make_float4(p0 - __log2f(d[0]), p1 - __log2f(d[1]), p2 - __log2f(d[2]), p3 - __log2f(d[3]));
+        reinterpret_cast<float4*>(s.f[h])[lane] = f;
+        if (lane == 0) {
+          *reinterpret_cast<float4*>(s.tot[h]) = make_float4(t0, t1, t2, t3);
+          s.decay[h] = ex2f(sum);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(B_SCAL + c % kScals));
+    }
+    if (!kFull && ok && mine > 0 && lane == 0) {
+      p.decays[2 * it.slot + h] = ex2f(log_decay);
+      if (kWide) p.decays[2 * it.slot + 1] = ex2f(log_decay);
+    }
   } else {
-    // ---- loads of x, stores of out -----------------------------------------------------------------------------------------------
-    const int column = it.head0 * (kWide ? 128 : 64);
+    // ---- tensor copies ------------------------------------------------------------------------------------------------------------
+    // They are worked off one behind the other, and a tile of out takes some 1400 cycles to leave.  So it goes behind the loads of B and
+    // C, for which the next block's first product waits; x, of which there are three tiles, comes long before it is wanted.
+    const int column = it.head0 * (kWide ? 128 : 64), bc_column = it.group * kNs, first = static_cast<int>(it.t0), batch = static_cast<int>(it.b);
+    const int most = blocks < p.stop_loads_after ? blocks : p.stop_loads_after;
+    int nb = 0, nc = 0, nx = 0;                                       // loads of B, C, x so far
+    auto row_of = [&](int n) { return first + (kFull ? n : blocks - 1 - n) * kQ; };      // (the first pass goes backwards)
+    auto load_x = [&] {
+      if (lane == 0) {
+        const uint32_t full = bar(B_FULL_X + nx % kXs);
+        mbar_arrive_expect_tx(full, kTileX);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) tma_load_3d(sbase + L::kX + (nx % kXs) * kTileX + i * (kTileX / 2), &maps.x, column + 64 * i, row_of(nx), batch, full);
+      }
+      ++nx;
+      __syncwarp();
+    };
+    auto load_bc = [&](const CUtensorMap* map, uint32_t to, int full, int& n) {
+      if (lane == 0) {
+        mbar_arrive_expect_tx(bar(full), L::kTile);
+#pragma unroll
+        for (int i = 0; i < kNs / 64; ++i) tma_load_3d(to + i * 16384, map, bc_column + 64 * i, row_of(n), batch, bar(full));
+      }
+      ++n;
+      __syncwarp();
+    };
     auto store = [&](int c) {
-      const int buf = c & 1;
-      if (!warp_wait(bar(B_OUT + buf), (c >> 1) & 1, abort_flag)) return false;
-      const uint32_t x = sbase + L::kX + buf * kTileX;
+      if (!warp_wait(bar(B_OUT + c % kXs), (c / kXs) & 1, abort_flag)) return false;
+      const uint32_t x = sbase + L::kX + (c % kXs) * kTileX;
       const int64_t left = it.tokens - static_cast<int64_t>(c) * kQ;
       if (p.packed && left < kQ) {
         // rows behind the sequence's end are somebody else's
@@ -589,71 +671,81 @@ __global__ void __launch_bounds__(kThreads, 1) ssm_scan_kernel(const __grid_cons
           const int row = i / pieces, piece = i % pieces;
           *reinterpret_cast<uint4*>(dst + row * p.os.token + piece * 8) = lds128(x + (piece >> 3) * (kTileX / 2) + row * 128 + (((piece & 7) ^ (row & 7)) << 4));
         }
-        return true;
-      }
-      if (lane == 0) {
-        const int row = static_cast<int>(it.t0) + c * kQ;
-        tma_store_3d(&maps.out, x, column, row, static_cast<int>(it.b));
-        if (kWide || it.two) tma_store_3d(&maps.out, x + kTileX / 2, column + 64, row, static_cast<int>(it.b));
+      } else if (lane == 0) {
+        tma_store_3d(&maps.out, x, column, first + c * kQ, batch);
+        if (kWide || it.two) tma_store_3d(&maps.out, x + kTileX / 2, column + 64, first + c * kQ, batch);
         bulk_commit();
-        bulk_wait_read0();
       }
       __syncwarp();
       return true;
     };
-    int issued = 0;
-    for (int c = 0; c < blocks && c < p.stop_loads_after; ++c) {
-      const int buf = c & 1;
-      if (c >= 2) {
-        ok = kFull ? store(c - 2) : warp_wait(bar(B_EMPTY_X + buf), ((c >> 1) - 1) & 1, abort_flag);
-        if (!ok) break;
-      }
-      if (lane == 0) {
-        mbar_arrive_expect_tx(bar(B_FULL_X + buf), kTileX);
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          tma_load_3d(sbase + L::kX + buf * kTileX + i * (kTileX / 2), &maps.x, column + 64 * i, static_cast<int>(it.t0) + c * kQ, static_cast<int>(it.b), bar(B_FULL_X + buf));
-      }
-      __syncwarp();
-      issued = c + 1;
+    if (most > 0) {
+      load_bc(&maps.b, sbase + L::kB, B_FULL_B, nb);
+      if constexpr (kFull) load_bc(&maps.c, sbase + L::kC, B_FULL_C, nc);
+      else if (nb < most) load_bc(&maps.b, sbase + L::kB + L::kTile, B_FULL_B + 1, nb);
+      while (nx < kXs && nx < most) load_x();
     }
-    if (kFull && ok)
-      for (int c = blocks > 2 ? blocks - 2 : 0; ok && c < blocks; ++c) ok = store(c);
+    for (int c = 0; c < blocks; ++c) {
+      if (c + 1 >= kXs && c + 1 < most) {
+        if constexpr (kFull) {
+          if (lane == 0) bulk_wait_read0();                           // (the output of block c - 2, which lay there)
+        } else {
+          if (!(ok = warp_wait(bar(B_EMPTY_X + nx % kXs), (nx / kXs - 1) & 1, abort_flag))) break;
+        }
+        load_x();
+      }
+      if constexpr (kFull) {
+        if (c + 1 < most) {
+          if (!(ok = warp_wait(bar(B_Z), c & 1, abort_flag))) break;
+          load_bc(&maps.c, sbase + L::kC, B_FULL_C, nc);
+          if (!(ok = warp_wait(bar(B_S_FULL), c & 1, abort_flag))) break;
+          load_bc(&maps.b, sbase + L::kB, B_FULL_B, nb);
+        }
+      } else if (c + 2 < most) {
+        if (!(ok = warp_wait(bar(B_EMPTY_B + (c & 1)), (c >> 1) & 1, abort_flag))) break;
+        load_bc(&maps.b, sbase + L::kB + (c & 1) * L::kTile, B_FULL_B + (c & 1), nb);
+      }
+      if (kFull && c > 0 && !(ok = store(c - 1))) break;
+    }
+    if (kFull && ok && blocks > 0) ok = store(blocks - 1);
+    // every copy has landed before this CTA's memory goes to another: those that nobody waited for
     if (lane == 0) {
       asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
-      for (int c = issued > 2 ? issued - 2 : 0; c < issued; ++c) drain(bar(B_FULL_X + (c & 1)), (c >> 1) & 1);
+      for (int c = nx > kXs ? nx - kXs : 0; c < nx; ++c) drain(bar(B_FULL_X + c % kXs), (c / kXs) & 1);
+      if constexpr (kFull) {
+        if (nb > 0) drain(bar(B_FULL_B), (nb - 1) & 1);
+        if (nc > 0) drain(bar(B_FULL_C), (nc - 1) & 1);
+      } else {
+        for (int c = nb > 2 ? nb - 2 : 0; c < nb; ++c) drain(bar(B_FULL_B + (c & 1)), (c >> 1) & 1);
+      }
     }
     __syncwarp();
   }
-  if ((!ok || *abort_flag > 0) && p.status != nullptr) atomicCAS(p.status, kStatusOk, kStatusWaitTimeout);
+  if (!ok) *abort_flag = 1;
   tc_fence_before();
   __syncthreads();
+  if (*abort_flag > 0 || p.queue == nullptr || !it.there) break;
+  }
+  if (tid == 0 && *abort_flag > 0) atomicCAS(p.status, kStatusOk, kStatusWaitTimeout);
   if (warp == 17) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc(tmem_base, 512);
   }
 }
 
 // ---- plan of a packed batch, and the chaining of runs -------------------------------------------------------------------------------
 // Sequences of more than kSsmStepT tokens, longest first, cut into runs of the length that the costs below (in blocks of the full walk) make cheapest.
-constexpr int kPlanThreads = 1024, kCandidates = 8;
+constexpr int kPlanThreads = 512, kPlanWarps = kPlanThreads / 32, kCandidates = 8;
 __device__ __forceinline__ int candidate(int least, int i) {         // run lengths that are tried; the last one: whole sequences
   return i == kCandidates - 1 ? 0x7fffffff : (least << (i >> 1)) + ((i & 1) ? (least << (i >> 1)) / 2 : 0);
 }
 __global__ void __launch_bounds__(kPlanThreads) ssm_plan_kernel(const int64_t* cu, int N, int64_t T, int pairs, int sms, int least, SsmPlan* plan, int* status) {
-  __shared__ int s_blocks[kSsmPlanMost];
-  __shared__ int s_seq[kSsmPlanMost];
-  __shared__ int s_active, s_longest, s_bad;
-  __shared__ unsigned long long s_total, s_first[kCandidates];
-  __shared__ int s_run;
+  __shared__ int s_blocks[kSsmPlanMost], s_seq[kSsmPlanMost];
+  __shared__ int s_sum[2][kPlanWarps], s_active, s_longest, s_bad, s_run, s_cut, s_total, s_first[kCandidates], s_cuts[kCandidates], s_runs[kCandidates];
   grid_dependency_wait();
-  const int tid = threadIdx.x;
-  if (tid == 0) {
-    s_active = s_longest = s_bad = 0;
-    s_total = 0;
-    if (status != nullptr) *status = 0;
-  }
-  if (tid < kCandidates) s_first[tid] = 0;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (tid == 0) s_active = s_longest = s_bad = s_cut = s_total = 0;
+  if (tid < kCandidates) s_first[tid] = s_cuts[tid] = s_runs[tid] = 0;
   __syncthreads();
   auto blocks_of = [&](int n) {
     int64_t bos = cu[n], eos = cu[n + 1];
@@ -663,16 +755,14 @@ __global__ void __launch_bounds__(kPlanThreads) ssm_plan_kernel(const int64_t* c
     return eos - bos <= kSsmStepT ? 0 : static_cast<int>((eos - bos + kQ - 1) / kQ);
   };
   // the sequences with blocks, in the order that they come in where they are too many to be sorted
-  int* order = plan->order(), *prefix = plan->prefix(N), *slots = plan->slot_prefix(N);
+  int *order = plan->order(), *prefix = plan->prefix(N), *slots = plan->slot_prefix(N);
   for (int base = 0; base < N; base += kPlanThreads) {
-    const int n = base + tid;
-    const int b = n < N ? blocks_of(n) : 0;
-    __shared__ int s_scan[32];
+    const int n = base + tid, b = n < N ? blocks_of(n) : 0;
     const unsigned vote = __ballot_sync(0xffffffffu, b > 0);
-    if ((tid & 31) == 0) s_scan[tid >> 5] = __popc(vote);
+    if (lane == 0) s_sum[0][warp] = __popc(vote);
     __syncthreads();
-    int at = s_active + __popc(vote & ((1u << (tid & 31)) - 1));
-    for (int i = 0; i < (tid >> 5); ++i) at += s_scan[i];
+    int at = s_active + __popc(vote & ((1u << lane) - 1));
+    for (int i = 0; i < warp; ++i) at += s_sum[0][i];
     if (b > 0) {
       if (at < N) order[at] = n;
       if (at < kSsmPlanMost) {
@@ -680,46 +770,49 @@ __global__ void __launch_bounds__(kPlanThreads) ssm_plan_kernel(const int64_t* c
         s_blocks[at] = b;
       }
       atomicMax(&s_longest, b);
-      atomicAdd(&s_total, static_cast<unsigned long long>(b));
-      if (least > 0)
-        for (int i = 0; i < kCandidates; ++i) {
-          const int l = candidate(least, i);
-          if (b > l) atomicAdd(&s_first[i], static_cast<unsigned long long>((b - 1) / l) * l);
+      atomicAdd(&s_total, b);
+      for (int i = 0; i < kCandidates - 1 && least > 0; ++i) {
+        const int l = candidate(least, i);
+        if (b > l) {
+          atomicAdd(&s_first[i], (b - 1) / l * l);
+          atomicAdd(&s_cuts[i], 1);
+          atomicAdd(&s_runs[i], (b - 1) / l + 1);
         }
+      }
     }
     __syncthreads();
-    if (tid == 0)
-      for (int i = 0; i < 32; ++i) s_active += s_scan[i];
+    if (tid < 32) {
+      int k = lane < kPlanWarps ? s_sum[0][lane] : 0;
+      for (int d = 16; d > 0; d >>= 1) k += __shfl_xor_sync(0xffffffffu, k, d);
+      if (lane == 0) s_active += k;
+    }
     __syncthreads();
   }
   // (sequences that are not monotone may overlap, and then be more than there is room for: none is walked)
   const int active = s_bad ? 0 : s_active;
-  if (tid == 0 && s_bad && status != nullptr) atomicCAS(status, kStatusOk, kStatusBadCuSeqlens);
   const bool sorted = active <= kSsmPlanMost;
-  if (tid == 0) {
-    int run = 0x7fffffff;
-    if (least > 0 && sorted) {
-      long long best = -1;
-      for (int i = kCandidates - 1; i >= 0; --i) {
-        const int l = candidate(least, i);
-        const long long even = static_cast<long long>(s_total * pairs + sms - 1) / sms, longest = s_longest < l ? s_longest : l;
-        long long cost = 100 * (even > longest ? even : longest) + 30 * (even < longest ? even : longest);
-        if (s_first[i] > 0) {
-          const long long first = static_cast<long long>(s_first[i] * pairs + sms - 1) / sms;
-          cost += kSsmFirstCost * (first > longest ? first : longest) + kSsmCutCost;
-        }
-        if (best < 0 || cost < best) {
-          best = cost;
-          run = l;
-        }
-      }
+  if (tid < 32) {
+    // the cheapest run length: the longest walk or an even share of all, whichever takes longer, and a little of the other; the same for
+    // the first pass, which takes the runs of cut sequences but their last ones; and the states between the passes
+    float cost = 3e38f;
+    if (lane < kCandidates && (lane == kCandidates - 1 || (least > 0 && sorted))) {
+      const int l = candidate(least, lane), cuts = lane < kCandidates - 1 ? s_cuts[lane] : 0, runs = lane < kCandidates - 1 ? s_runs[lane] : 0;
+      const float share = static_cast<float>(pairs) / sms, longest = s_longest < l ? s_longest : l;
+      auto both = [](float a, float b) { return fmaxf(a, b) + 0.15f * fminf(a, b); };
+      cost = both((100.f * s_total + kSsmStartCost * (active - cuts + runs)) * share, 100.f * longest + kSsmStartCost);
+      if (cuts > 0) cost += both((kSsmFirstCost * s_first[lane] + kSsmStartCost * (runs - cuts)) * share, kSsmFirstCost * longest + kSsmStartCost) + kSsmChainCost + kSsmSlotCost * 0.01f * runs * pairs;
     }
-    s_run = run;
-    plan->run_blocks = run;
-    plan->active = active;
+    float best = cost;
+    for (int d = 16; d > 0; d >>= 1) best = fminf(best, __shfl_xor_sync(0xffffffffu, best, d));
+    const unsigned at = __ballot_sync(0xffffffffu, cost == best);
+    if (lane == 0) {
+      s_run = candidate(least, 31 - __clz(at));                        // (of equal ones the longest)
+      plan->run_blocks = s_run;
+      plan->active = active;
+      plan->next[0] = plan->next[1] = 0;
+      if (status != nullptr) *status = s_bad ? kStatusBadCuSeqlens : 0;
+    }
   }
-  __syncthreads();
-  const int run = s_run;
   if (sorted) {
     for (int i = tid; i < active; i += kPlanThreads) {
       const int b = s_blocks[i];
@@ -727,43 +820,41 @@ __global__ void __launch_bounds__(kPlanThreads) ssm_plan_kernel(const int64_t* c
       for (int k = 0; k < active; ++k) rank += s_blocks[k] > b || (s_blocks[k] == b && k < i);
       order[rank] = s_seq[i];
     }
-    __syncthreads();
   }
+  __syncthreads();
+  const int run = s_run;
   // prefixes over the ranks: runs, and runs of the sequences that are cut (they come first)
-  __shared__ int s_part[2][32];
   int done[2] = {0, 0};
   for (int base = 0; base < active; base += kPlanThreads) {
     const int i = base + tid;
     int runs = 0;
-    if (i < active) {
-      const int b = blocks_of(order[i]);
-      runs = run == 0x7fffffff ? 1 : (b + run - 1) / run;
-    }
+    if (i < active) runs = run == 0x7fffffff ? 1 : (blocks_of(order[i]) + run - 1) / run;
     int a = runs, c = runs > 1 ? runs : 0;
     for (int d = 1; d < 32; d <<= 1) {
       const int u = __shfl_up_sync(0xffffffffu, a, d), v = __shfl_up_sync(0xffffffffu, c, d);
-      if ((tid & 31) >= d) {
+      if (lane >= d) {
         a += u;
         c += v;
       }
     }
-    if ((tid & 31) == 31) {
-      s_part[0][tid >> 5] = a;
-      s_part[1][tid >> 5] = c;
+    if (lane == 31) {
+      s_sum[0][warp] = a;
+      s_sum[1][warp] = c;
     }
     __syncthreads();
     int whole[2] = {0, 0};
-    for (int k = 0; k < 32; ++k) {
-      if (k < (tid >> 5)) {
-        a += s_part[0][k];
-        c += s_part[1][k];
+    for (int k = 0; k < kPlanWarps; ++k) {
+      if (k < warp) {
+        a += s_sum[0][k];
+        c += s_sum[1][k];
       }
-      whole[0] += s_part[0][k];
-      whole[1] += s_part[1][k];
+      whole[0] += s_sum[0][k];
+      whole[1] += s_sum[1][k];
     }
     if (i < active) {
       prefix[i + 1] = done[0] + a;
       slots[i + 1] = done[1] + c;
+      if (runs > 1) atomicMax(&s_cut, i + 1);
     }
     done[0] += whole[0];
     done[1] += whole[1];
@@ -771,21 +862,19 @@ __global__ void __launch_bounds__(kPlanThreads) ssm_plan_kernel(const int64_t* c
   }
   if (tid == 0) {
     prefix[0] = slots[0] = 0;
-    plan->cut = 0;
+    plan->cut = s_cut;
   }
-  __syncthreads();
-  for (int i = tid; i < active; i += kPlanThreads)
-    if (slots[i + 1] > slots[i]) atomicMax(&plan->cut, i + 1);
 }
 
 // Per sequence that is cut: its runs' local states -> the state that each run starts from.
 __global__ void __launch_bounds__(256) ssm_chain_kernel(const SsmScanParams p, int Ns, int pairs) {
   grid_dependency_wait();
   const int pieces = 128 * Ns / 4 / 256;                              // blocks of 256 float4
-  const int piece = static_cast<int>(blockIdx.x % pieces), pair = static_cast<int>(blockIdx.x / pieces % pairs), rank = static_cast<int>(blockIdx.x / pieces / pairs);
+  const int piece = static_cast<int>(blockIdx.x % pieces), pair = static_cast<int>(blockIdx.x / pieces % pairs);
+  const int stride = static_cast<int>(gridDim.x / pieces / pairs), ranks = p.packed ? p.plan->cut : p.N;
+  for (int rank = static_cast<int>(blockIdx.x / pieces / pairs); rank < ranks; rank += stride) {
   int n = rank, runs = p.runs, first = rank * p.runs;
   if (p.packed) {
-    if (rank >= p.plan->cut) return;
     n = p.plan->order()[rank];
     first = p.plan->slot_prefix(p.N)[rank];
     runs = p.plan->slot_prefix(p.N)[rank + 1] - first;
@@ -804,16 +893,27 @@ __global__ void __launch_bounds__(256) ssm_chain_kernel(const SsmScanParams p, i
       s = make_float4(bf_lo(w.x), bf_hi(w.x), bf_lo(w.y), bf_hi(w.y));
     }
   }
-  float4 next = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int r = 0; r < runs; ++r) {
-    const int64_t slot = static_cast<int64_t>(first + r) * pairs + pair;
-    float4* q = reinterpret_cast<float4*>(p.slots + slot * 128 * Ns + at);
-    if (r + 1 < runs) next = *q;
-    *q = s;
-    if (r + 1 < runs) {
-      const float d = p.decays[2 * slot + h];
-      s = make_float4(fmaf(d, s.x, next.x), fmaf(d, s.y, next.y), fmaf(d, s.z, next.z), fmaf(d, s.w, next.w));
+  // (eight runs' states and decays on their way at a time: one behind the other, a run takes 1.9 us)
+  constexpr int kAhead = 8;
+  for (int r0 = 0; r0 < runs; r0 += kAhead) {
+    float4 local[kAhead];
+    float d[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int64_t slot = static_cast<int64_t>(first + r0 + i) * pairs + pair;
+      if (r0 + i + 1 < runs) {
+        local[i] = *reinterpret_cast<const float4*>(p.slots + slot * 128 * Ns + at);
+        d[i] = p.decays[2 * slot + h];
+      }
     }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if (r0 + i >= runs) break;
+      const int64_t slot = static_cast<int64_t>(first + r0 + i) * pairs + pair;
+      *reinterpret_cast<float4*>(p.slots + slot * 128 * Ns + at) = s;
+      if (r0 + i + 1 < runs) s = make_float4(fmaf(d[i], s.x, local[i].x), fmaf(d[i], s.y, local[i].y), fmaf(d[i], s.z, local[i].z), fmaf(d[i], s.w, local[i].w));
+    }
+  }
   }
 }
 
@@ -835,7 +935,8 @@ cudaError_t launch_walk(const SsmMaps& maps, const SsmScanParams& p, int64_t ite
   auto kernel = ssm_scan_kernel<kNs, kWide, kFull>;
   const cudaError_t e = opt_in.ensure(kernel, Smem<kNs>::kBytes);
   if (e != cudaSuccess) return e;
-  return launch_after(kernel, dim3(static_cast<unsigned>(items)), kThreads, Smem<kNs>::kBytes, stream, maps, p);
+  const int64_t ctas = p.queue != nullptr && items > device_sm_count() ? device_sm_count() : items;
+  return launch_after(kernel, dim3(static_cast<unsigned>(ctas)), kThreads, Smem<kNs>::kBytes, stream, maps, p);
 }
 template <bool kFull>
 cudaError_t launch_pass(const SsmMaps& maps, const SsmScanParams& p, int Ns, int64_t items, cudaStream_t stream) {
@@ -853,13 +954,14 @@ SsmLayout ssm_layout(int64_t T, int64_t N, int H, int P, int G, int Ns, bool pac
   if (!packed) {
     const int64_t blocks = (T + kSsmBlock - 1) / kSsmBlock, chains = N * L.pairs;
     auto rounds = [&](int64_t ctas) { return (ctas + sms - 1) / sms; };
-    int64_t best = rounds(chains) * blocks * 100;
+    int64_t best = rounds(chains) * (blocks * 100 + kSsmStartCost);
     L.runs = 1;
     L.run_blocks = static_cast<int>(blocks);
     for (int64_t r = 2; r <= blocks && r <= 160 && chains < 4 * sms; ++r) {
       const int64_t len = (blocks + r - 1) / r;
       if ((r - 1) * len >= blocks) continue;                        // the last run would be empty
-      const int64_t cost = (rounds(chains * r) * 100 + rounds(chains * (r - 1)) * kSsmFirstCost) * len + kSsmCutCost + kSsmRunCost * r;
+      const int64_t cost = rounds(chains * r) * (len * 100 + kSsmStartCost) + rounds(chains * (r - 1)) * (len * kSsmFirstCost + kSsmStartCost) + kSsmChainCost +
+                           kSsmSlotCost * chains * r / 100;
       if (cost < best) {
         best = cost;
         L.runs = static_cast<int>(r);
@@ -925,19 +1027,26 @@ cudaError_t launch_ssm_scan(const SsmParams& q, const SsmLayout& L, const SsmAid
   p.run_blocks = L.run_blocks;
   p.packed = packed;
   p.state_fp32 = q.state_fp32;
-  p.split = q.final_state != nullptr && q.state_fp32;
   p.wait_limit_us = aid.wait_limit_us;
   p.stop_loads_after = aid.stop_loads_after > 0 ? aid.stop_loads_after : 0x7fffffff;
   cudaError_t e = cudaSuccess;
-  if (packed) e = launch_after(ssm_scan::ssm_plan_kernel, dim3(1), ssm_scan::kPlanThreads, 0, stream, q.cu_seqlens, q.N, q.T, L.pairs, device_sm_count(), L.least, p.plan, p.status);
-  else if (clear_status) e = cudaMemsetAsync(ws, 0, 4, stream);
+  if (packed) {
+    e = launch_after(ssm_scan::ssm_plan_kernel, dim3(1), ssm_scan::kPlanThreads, 0, stream, q.cu_seqlens, q.N, q.T, L.pairs, device_sm_count(), L.least, p.plan, p.status);
+    // the sequences of a few tokens, decode steps among the prompts
+    if (e == cudaSuccess) e = launch_ssm_step(q, kSsmStepT, stream);
+  } else if (clear_status) {
+    e = cudaMemsetAsync(ws, 0, 4, stream);
+  }
   if (e != cudaSuccess) return e;
   if (L.first_items > 0) {
+    if (packed) p.queue = p.plan->next;
     e = ssm_scan::launch_pass<false>(maps, p, q.Ns, L.first_items, stream);
     if (e != cudaSuccess) return e;
-    e = launch_after(ssm_scan::ssm_chain_kernel, dim3(static_cast<unsigned>(L.chained * L.pairs * (128 * q.Ns / 1024))), 256, 0, stream, p, q.Ns, L.pairs);
+    const int64_t each = L.pairs * (128 * q.Ns / 1024), most = (8 * device_sm_count() + each - 1) / each;
+    e = launch_after(ssm_scan::ssm_chain_kernel, dim3(static_cast<unsigned>(each * (L.chained < most ? L.chained : most))), 256, 0, stream, p, q.Ns, L.pairs);
     if (e != cudaSuccess) return e;
   }
+  if (packed) p.queue = p.plan->next + 1;
   return ssm_scan::launch_pass<true>(maps, p, q.Ns, L.items, stream);
 }
 

@@ -18,9 +18,6 @@ using elem::pk;
 
 constexpr int kThreads = 128;
 
-// softplus to fp32 accuracy: max(x, 0) + log(1 + e^-|x|)
-__device__ __forceinline__ float softplus(float x) { return fmaxf(x, 0.f) + log1pf(ex2f(-kLog2e * fabsf(x))); }
-
 template <int kNs, bool kFp32, bool kPacked>
 __global__ void __launch_bounds__(kThreads) ssm_step_kernel(const SsmParams p, int most) {
   constexpr int kLanes = kNs / 8, kRows = 4 * (32 / kLanes) * (kThreads / 32);

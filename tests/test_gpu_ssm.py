@@ -43,8 +43,9 @@ def exponent_slack(A_log, dt, dt_bias, lens):
 
 def check(got, fin, want, mass, last, lmass, longest, lens_rows, state_bf16, slack):
     """`out`: one rounding to bf16; where the scan goes in blocks, the products C B^T (with decay) and the state are operands
-    rounded to bf16, half a step each of every term.  fp32: sums of up to 128 + Ns terms per block and the exponents.  The state is a sum of terms whose
-    operand is split in two bf16 parts (2^-16 of a term) and is rescaled once per block in fp32."""
+    rounded to bf16, half a step each of every term.  fp32: sums of up to 128 + Ns terms per block and the exponents.  The state is a sum of terms x w B with
+    w and x w each split in two bf16 parts: 2^-16 of a term for what w loses, and half a step of a second part that is at most 2^-7 of the term, 2^-15; it is
+    rescaled once per block in fp32."""
     blocks = max(1, -(-longest // 128))
     single = (400 + 4 * blocks) * R.FP32 + slack
     operands = 0.0 if longest <= STEP else 2 * R.BF16
@@ -53,7 +54,7 @@ def check(got, fin, want, mass, last, lmass, longest, lens_rows, state_bf16, sla
     if longest > STEP:
         assert ((got.double().cpu() - want).norm() / want.norm().clamp_min(1e-30)).item() <= 3 * R.BF16
     if fin is not None:
-        split = 0.0 if longest <= STEP else R.BF16 if state_bf16 else 2.0 ** -16
+        split = 0.0 if longest <= STEP else 3 * 2.0 ** -16
         assert R.off(fin, last, (R.BF16 if state_bf16 else R.FP32) * last.abs() + (split + single) * lmass + 1e-30) <= 1
 
 
