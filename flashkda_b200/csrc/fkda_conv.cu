@@ -1,25 +1,43 @@
 // Depthwise causal convolution of 2 to 4 taps with bias and SiLU, over prompts, packed batches and single tokens.
 //
-// y[t][c] = act(bias[c] + sum_k w[c][k] x[t - (W-1) + k][c]).  A thread owns eight channels (16 bytes) and walks a tile of tokens with
+// y[t][c] = act(bias[c] + sum_k w[c][k] x[t - (W-1) + k][c]).  A thread owns four channels (8 bytes) and walks a tile of tokens with
 // the last W-1 inputs in registers, so that every input is read from memory once, but for the W-1 rows before each tile.
 // States: the last W-1 inputs of a sequence.  Only the thread that owns a sequence's first token reads the initial state, and it
 // writes the final one behind that (from the sequence's last rows), so the two may be one tensor; for that it also walks the tokens
 // behind its tile that still see the initial state, which the next tile leaves out.
+#include "fkda_elem.cuh"
 #include "fkda_layer.cuh"
 
 namespace fkda {
 namespace conv {
 
-constexpr int kThreads = 128;
-constexpr int kGroup = 4;          // tokens whose loads are in flight together
+using elem::f2;
+using elem::fma2;
+using elem::mul;
+using elem::pk;
 
-template <int W, bool kWFp32, bool kPacked>
-__global__ void __launch_bounds__(kThreads) conv_kernel(const ConvParams p) {
+constexpr int kThreads = 128;
+constexpr int kOwn = 4;            // channels of a thread
+constexpr int kGroup = 4;          // tokens whose loads are in flight together, while those of the group before are worked on
+
+__device__ __forceinline__ void unpack(const uint2& v, f2 (&x)[2]) {
+  x[0] = pk(bf_lo(v.x), bf_hi(v.x));
+  x[1] = pk(bf_lo(v.y), bf_hi(v.y));
+}
+__device__ __forceinline__ f2 silu(f2 y) {
+  float a, b;
+  elem::upk(mul(y, pk(-kLog2e, -kLog2e)), a, b);
+  elem::upk(elem::add2(pk(ex2f(a), ex2f(b)), pk(1.f, 1.f)), a, b);
+  return mul(y, pk(rcpf(a), rcpf(b)));
+}
+
+template <int W, bool kWFp32, bool kPacked, bool kSilu>
+__global__ void __launch_bounds__(kThreads, 5) conv_kernel(const ConvParams p) {
   grid_dependency_wait();
-  const unsigned vecs = static_cast<unsigned>(p.C) / 8;
+  const unsigned vecs = static_cast<unsigned>(p.C) / kOwn;
   const int64_t flat = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
   const int64_t item = flat / vecs;
-  const int c = static_cast<int>(flat - item * vecs) * 8;
+  const int c = static_cast<int>(flat - item * vecs) * kOwn;
   const int64_t items = static_cast<int64_t>(kPacked ? 1 : p.N) * p.tiles;
   if (item >= items) {
     // one more thread per sequence and channel vector, where there may be sequences without tokens: hands their state on
@@ -27,9 +45,9 @@ __global__ void __launch_bounds__(kThreads) conv_kernel(const ConvParams p) {
     if (p.final_state == nullptr || n >= p.N || (kPacked ? p.cu_seqlens[n + 1] > p.cu_seqlens[n] : p.T > 0)) return;
     for (int j = 0; j < W - 1; ++j) {
       const int64_t at = (n * (W - 1) + j) * p.C + c;
-      uint4 v = make_uint4(0u, 0u, 0u, 0u);
-      if (p.initial_state != nullptr) v = *reinterpret_cast<const uint4*>(p.initial_state + at);
-      *reinterpret_cast<uint4*>(p.final_state + at) = v;
+      uint2 v = make_uint2(0u, 0u);
+      if (p.initial_state != nullptr) v = *reinterpret_cast<const uint2*>(p.initial_state + at);
+      *reinterpret_cast<uint2*>(p.final_state + at) = v;
     }
     return;
   }
@@ -58,20 +76,39 @@ __global__ void __launch_bounds__(kThreads) conv_kernel(const ConvParams p) {
   if (bos > t) t = bos;                           // (rows before the first sequence)
   if (bos < t0 && t < bos + W - 1) t = bos + W - 1 < eos ? bos + W - 1 : eos;
 
-  float w[8 * W], b[8];
+  f2 w[W][2], b[2];                               // pairs of channels
+  {
+    float all[kOwn * W];
 #pragma unroll
-  for (int i = 0; i < W; ++i) {
-    float part[8];
-    load8<kWFp32>(p.weight, static_cast<int64_t>(c) * W + 8 * i, part);
+    for (int i = 0; i < W; ++i) {
+      const float4 v = load4<kWFp32>(p.weight, static_cast<int64_t>(c) * W + 4 * i);
+      all[4 * i] = v.x;
+      all[4 * i + 1] = v.y;
+      all[4 * i + 2] = v.z;
+      all[4 * i + 3] = v.w;
+    }
+    const float4 v = p.bias != nullptr ? load4<kWFp32>(p.bias, c) : make_float4(0.f, 0.f, 0.f, 0.f);
+    const float bias[kOwn] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int e = 0; e < 8; ++e) w[8 * i + e] = part[e];
+    for (int e = 0; e < 2; ++e) {
+      b[e] = pk(bias[2 * e], bias[2 * e + 1]);
+#pragma unroll
+      for (int j = 0; j < W; ++j) w[j][e] = pk(all[2 * e * W + j], all[(2 * e + 1) * W + j]);
+    }
   }
+  f2 u[W - 1 + kGroup][2];                        // the inputs that reach back, then a group's own
+  auto result = [&](int i) {
+    f2 y[2];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) b[e] = 0.f;
-  if (p.bias != nullptr) load8<kWFp32>(p.bias, c, b);
-
-  float past[W - 1][8];
-  bool fresh = true;                              // `past` has to be loaded
+    for (int e = 0; e < 2; ++e) {
+      y[e] = b[e];
+#pragma unroll
+      for (int j = 0; j < W; ++j) y[e] = fma2(w[j][e], u[i + j][e], y[e]);
+      if constexpr (kSilu) y[e] = silu(y[e]);
+    }
+    return make_uint2(elem::round_bf(y[0]), elem::round_bf(y[1]));
+  };
+  bool fresh = true;                              // what reaches back has to be loaded
   while (true) {
     if (t >= eos) {
       if constexpr (!kPacked) break;
@@ -95,64 +132,73 @@ __global__ void __launch_bounds__(kThreads) conv_kernel(const ConvParams p) {
 #pragma unroll
       for (int j = 0; j < W - 1; ++j) {
         const int64_t at = t - (W - 1) + j;
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (at >= bos) v = *reinterpret_cast<const uint4*>(x + at * p.xs.token);
-        else if (p.initial_state != nullptr) v = *reinterpret_cast<const uint4*>(p.initial_state + (n * (W - 1) + (W - 1) + at - bos) * p.C + c);
-        unpack8(v, past[j]);
+        uint2 v = make_uint2(0u, 0u);
+        if (at >= bos) v = *reinterpret_cast<const uint2*>(x + at * p.xs.token);
+        else if (p.initial_state != nullptr) v = *reinterpret_cast<const uint2*>(p.initial_state + (n * (W - 1) + (W - 1) + at - bos) * p.C + c);
+        unpack(v, u[j]);
       }
       if (t == bos && p.final_state != nullptr) {
-        uint4 last[W - 1];
+        uint2 last[W - 1];
 #pragma unroll
         for (int j = 0; j < W - 1; ++j) {
           const int64_t at = eos - (W - 1) + j;
-          last[j] = make_uint4(0u, 0u, 0u, 0u);
-          if (at >= bos) last[j] = *reinterpret_cast<const uint4*>(x + at * p.xs.token);
-          else if (p.initial_state != nullptr) last[j] = *reinterpret_cast<const uint4*>(p.initial_state + (n * (W - 1) + (W - 1) + at - bos) * p.C + c);
+          last[j] = make_uint2(0u, 0u);
+          if (at >= bos) last[j] = *reinterpret_cast<const uint2*>(x + at * p.xs.token);
+          else if (p.initial_state != nullptr) last[j] = *reinterpret_cast<const uint2*>(p.initial_state + (n * (W - 1) + (W - 1) + at - bos) * p.C + c);
         }
 #pragma unroll
-        for (int j = 0; j < W - 1; ++j) *reinterpret_cast<uint4*>(p.final_state + (n * (W - 1) + j) * p.C + c) = last[j];
+        for (int j = 0; j < W - 1; ++j) *reinterpret_cast<uint2*>(p.final_state + (n * (W - 1) + j) * p.C + c) = last[j];
       }
     }
-    for (; t < limit; t += kGroup) {
-      uint4 in[kGroup];
+    const __nv_bfloat16* from = x + t * p.xs.token;
+    __nv_bfloat16* to = out + t * p.os.token;
+    uint2 in[kGroup];
+    int left = static_cast<int>(limit - t);
+    if (left >= kGroup) {
 #pragma unroll
-      for (int i = 0; i < kGroup; ++i)
-        if (t + i < limit) in[i] = *reinterpret_cast<const uint4*>(x + (t + i) * p.xs.token);
+      for (int i = 0; i < kGroup; ++i) in[i] = *reinterpret_cast<const uint2*>(from + i * p.xs.token);
+    }
+    for (; left >= kGroup; left -= kGroup) {
 #pragma unroll
-      for (int i = 0; i < kGroup; ++i) {
-        if (t + i >= limit) break;
-        float now[8], y[8];
-        unpack8(in[i], now);
+      for (int i = 0; i < kGroup; ++i) unpack(in[i], u[W - 1 + i]);
+      from += kGroup * p.xs.token;
+      if (left >= 2 * kGroup) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          y[e] = b[e];
-#pragma unroll
-          for (int j = 0; j < W - 1; ++j) y[e] = fmaf(w[e * W + j], past[j][e], y[e]);
-          y[e] = fmaf(w[e * W + W - 1], now[e], y[e]);
-#pragma unroll
-          for (int j = 0; j + 1 < W - 1; ++j) past[j][e] = past[j + 1][e];
-          past[W - 2][e] = now[e];
-        }
-        if (p.silu) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) y[e] *= sigmoid_exact(y[e]);
-        }
-        *reinterpret_cast<uint4*>(out + (t + i) * p.os.token) = pack8(y);
+        for (int i = 0; i < kGroup; ++i) in[i] = *reinterpret_cast<const uint2*>(from + i * p.xs.token);
       }
+#pragma unroll
+      for (int i = 0; i < kGroup; ++i) *reinterpret_cast<uint2*>(to + i * p.os.token) = result(i);
+      to += kGroup * p.os.token;
+#pragma unroll
+      for (int j = 0; j < W - 1; ++j)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) u[j][e] = u[kGroup + j][e];
+    }
+    for (; left > 0; --left) {                  // (what is left of a group)
+      unpack(*reinterpret_cast<const uint2*>(from), u[W - 1]);
+      *reinterpret_cast<uint2*>(to) = result(0);
+      from += p.xs.token;
+      to += p.os.token;
+#pragma unroll
+      for (int j = 0; j < W - 1; ++j)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) u[j][e] = u[j + 1][e];
     }
     t = limit;
     if (t >= end && t < eos) break;
   }
 }
 
+template <int W, bool kWFp32, bool kPacked>
+auto pick(bool silu) { return silu ? conv_kernel<W, kWFp32, kPacked, true> : conv_kernel<W, kWFp32, kPacked, false>; }
+
 template <int W>
 cudaError_t launch(const ConvParams& p, bool weight_fp32, cudaStream_t stream) {
   const bool packed = p.cu_seqlens != nullptr;
   const int64_t items = (packed ? 1 : static_cast<int64_t>(p.N)) * p.tiles + (p.final_state != nullptr && (packed || p.T == 0) ? p.N : 0);
-  const int64_t blocks = (items * (p.C / 8) + kThreads - 1) / kThreads;
+  const int64_t blocks = (items * (p.C / kOwn) + kThreads - 1) / kThreads;
   if (blocks == 0) return cudaSuccess;
-  auto kernel = packed ? (weight_fp32 ? conv_kernel<W, true, true> : conv_kernel<W, false, true>)
-                       : (weight_fp32 ? conv_kernel<W, true, false> : conv_kernel<W, false, false>);
+  auto kernel = packed ? (weight_fp32 ? pick<W, true, true>(p.silu) : pick<W, false, true>(p.silu)) : (weight_fp32 ? pick<W, true, false>(p.silu) : pick<W, false, false>(p.silu));
   return launch_after(kernel, dim3(static_cast<unsigned>(blocks)), kThreads, 0, stream, p);
 }
 
@@ -160,10 +206,10 @@ cudaError_t launch(const ConvParams& p, bool weight_fp32, cudaStream_t stream) {
 
 cudaError_t launch_short_conv(ConvParams p, int width, bool weight_fp32, cudaStream_t stream) {
   const bool packed = p.cu_seqlens != nullptr;
-  const int64_t vectors = static_cast<int64_t>(packed ? 1 : p.N) * p.T * (p.C / 8);
-  // Tokens per thread: as many as leave every SM two thousand threads (the rows before a tile are read again, 3 of 16), but no
+  const int64_t vectors = static_cast<int64_t>(packed ? 1 : p.N) * p.T * (p.C / conv::kOwn);
+  // Tokens per thread: as many as leave every SM two thousand threads (the rows before a tile are read again, 3 of 64, and its weights), but no
   // fewer than the taps that reach back: only a sequence's first tile may see its initial state.
-  int tile = 16;
+  int tile = 64;
   while (tile > 4 && vectors / tile < 2048ll * device_sm_count()) tile >>= 1;
   p.tile = !packed && p.T < tile ? static_cast<int>(p.T > 0 ? p.T : 1) : tile;
   p.tiles = static_cast<int>((p.T + p.tile - 1) / p.tile);

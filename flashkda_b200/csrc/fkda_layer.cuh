@@ -53,8 +53,8 @@ struct GatedNormParams {
   const void* weight;
   __nv_bfloat16* out;
   Rows xs, gs, os;
-  int64_t rows;             // B T H
-  int64_t T;
+  int64_t rows;             // B T H, below 2^31
+  int64_t T;                // tokens of a batch row, or more than there are: batch rows follow one another
   int H, D;
   float eps;
   int per_head;
@@ -68,8 +68,8 @@ struct AddNormParams {
   __nv_bfloat16* out;
   void* residual_out;
   Rows xs, rs, os, ros;
-  int64_t rows;             // B T
-  int64_t T;
+  int64_t rows;             // B T, below 2^31
+  int64_t T;                // as above
   int D;
   float scale, eps;
 };
@@ -89,8 +89,20 @@ __device__ __forceinline__ void load8(const void* base, int64_t at, float (&w)[8
     unpack8(__ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(base) + at)), w);
   }
 }
+// Four consecutive weights as fp32.
+template <bool kFp32>
+__device__ __forceinline__ float4 load4(const void* base, int64_t at) {
+  if constexpr (kFp32) return __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(base) + at));
+  const uint2 v = __ldg(reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(base) + at));
+  return make_float4(bf_lo(v.x), bf_hi(v.x), bf_lo(v.y), bf_hi(v.y));
+}
+__device__ __forceinline__ float rcpf(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 // 1 / (1 + e^-x) to fp32 accuracy (the tanh approximation has an absolute error that small values do not bear)
-__device__ __forceinline__ float sigmoid_exact(float x) { return __fdividef(1.f, 1.f + ex2f(-kLog2e * x)); }
+__device__ __forceinline__ float sigmoid_exact(float x) { return rcpf(1.f + ex2f(-kLog2e * x)); }
 
 // max(x, 0) + log(1 + e^-|x|) to fp32 accuracy.  log(1 + u) = 2 atanh(z) with z = u / (2 + u) <= 1/3, by the series of atanh to z^13: what is
 // left out is below 2^-26 of the sum.

@@ -1,5 +1,6 @@
 // C ABI of the operators round the recurrence (include/fkda.h): argument checks and launches.
 #include <cmath>
+#include <initializer_list>
 
 #include "../../include/fkda.h"
 #include "../../include/fkda_testing.h"
@@ -90,8 +91,14 @@ int64_t span(const View& v, const Sizes& s) {
   return ((r.B - 1) * r.batch + (r.T - 1) * r.token + v.inner) * v.size;
 }
 Rows rows_of(const View& v, const Sizes& s) {
-  // (strides of dimensions with one entry may be anything; the kernels multiply them by 0)
-  return Rows{s.B > 1 ? v.batch : 0, s.T > 1 ? v.token : 0};
+  // (strides of dimensions with one entry may be anything; the kernels multiply those by 0)
+  return Rows{s.B > 1 ? v.batch : 0, s.T > 1 ? v.token : s.B > 1 && s.T == 1 ? v.batch : 0};
+}
+// Tokens of a batch row as the norms count them: all of them where every batch row follows the one before (no division then).
+int64_t tokens_of(const Sizes& s, std::initializer_list<Rows> tensors) {
+  for (const Rows& r : tensors)
+    if (s.B > 1 && r.batch != s.T * r.token) return s.T;
+  return INT64_MAX;
 }
 bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 bool known(int32_t dtype) { return dtype == FKDA_STATE_BF16 || dtype == FKDA_STATE_FP32; }
@@ -279,7 +286,7 @@ int fkda_gated_norm(const fkda_gated_norm_params* p, void* cuda_stream) {
     if (share(*v, o, s) && !same(*v, o, s)) return set_error(FKDA_ERR_INVALID_ARGUMENT, "out shares memory with %s without being it", v->name);
   if (over(o, s, p->weight, (p->weight_per_head ? p->H : 1) * p->D, p->weight_dtype)) return refuse("out shares memory with weight");
   const fkda::GatedNormParams q{static_cast<const __nv_bfloat16*>(p->x), static_cast<const __nv_bfloat16*>(p->gate), p->weight, static_cast<__nv_bfloat16*>(p->out),
-                                rows_of(x, s), rows_of(g, s), rows_of(o, s), p->B * p->T * p->H, p->T, static_cast<int>(p->H), static_cast<int>(p->D), p->eps,
+                                rows_of(x, s), rows_of(g, s), rows_of(o, s), p->B * p->T * p->H, tokens_of(s, {rows_of(x, s), rows_of(g, s), rows_of(o, s)}), static_cast<int>(p->H), static_cast<int>(p->D), p->eps,
                                 p->weight_per_head != 0};
   const cudaError_t e = fkda::launch_gated_norm(q, p->weight_dtype == FKDA_STATE_FP32, p->silu != 0, p->gate_first != 0, static_cast<cudaStream_t>(cuda_stream));
   return e == cudaSuccess ? FKDA_OK : cuda_error(e, "gated norm launch");
@@ -306,7 +313,7 @@ int fkda_add_norm(const fkda_add_norm_params* p, void* cuda_stream) {
   if (share(x, ro, s)) return refuse("residual_out shares memory with x");
   if (over(o, s, p->weight, p->D, p->weight_dtype) || over(ro, s, p->weight, p->D, p->weight_dtype)) return refuse("an output shares memory with weight");
   const fkda::AddNormParams q{static_cast<const __nv_bfloat16*>(p->x), p->residual, p->weight, static_cast<__nv_bfloat16*>(p->out), p->residual_out,
-                              rows_of(x, s), rows_of(r, s), rows_of(o, s), rows_of(ro, s), p->B * p->T, p->T, static_cast<int>(p->D), p->scale, p->eps};
+                              rows_of(x, s), rows_of(r, s), rows_of(o, s), rows_of(ro, s), p->B * p->T, tokens_of(s, {rows_of(x, s), rows_of(r, s), rows_of(o, s), rows_of(ro, s)}), static_cast<int>(p->D), p->scale, p->eps};
   const cudaError_t e = fkda::launch_add_norm(q, p->weight_dtype == FKDA_STATE_FP32, p->residual_dtype == FKDA_STATE_FP32, static_cast<cudaStream_t>(cuda_stream));
   return e == cudaSuccess ? FKDA_OK : cuda_error(e, "residual norm launch");
 }

@@ -5,6 +5,7 @@
 //
 // One pass: a row lives in the registers of the threads that share it, eight elements (16 bytes of bf16) at a time, from its loads to its
 // stores; the sum of squares is fp32.  Rows of up to 1024 elements are shared by 8 to 32 lanes of a warp, longer ones by a block.
+#include "fkda_elem.cuh"
 #include "fkda_layer.cuh"
 
 namespace fkda {
@@ -48,59 +49,97 @@ __device__ __forceinline__ Place place(int64_t rows, int lanes) {
   if (!w.live) w.row = rows - 1;               // (takes part in the sums, stores nothing)
   return w;
 }
-__device__ __forceinline__ int64_t at_token(const Rows& s, int64_t token, int64_t T) {
-  const int64_t b = token / T;
-  return b * s.batch + (token - b * T) * s.token;
+__device__ __forceinline__ int64_t at_token(const Rows& s, unsigned token, int64_t T) {
+  if (T > 0x7fffffff) return token * s.token;                      // (one row of tokens)
+  const unsigned b = token / static_cast<unsigned>(T);
+  return b * s.batch + (token - b * static_cast<unsigned>(T)) * s.token;
 }
 
-template <bool kBlock, int V, bool kWFp32, bool kSilu, bool kFirst>
+using elem::f2;
+using elem::fma2;
+using elem::mul;
+using elem::pk;
+__device__ __forceinline__ void unpack(const uint4& v, f2 (&x)[4]) {
+  x[0] = pk(bf_lo(v.x), bf_hi(v.x));
+  x[1] = pk(bf_lo(v.y), bf_hi(v.y));
+  x[2] = pk(bf_lo(v.z), bf_hi(v.z));
+  x[3] = pk(bf_lo(v.w), bf_hi(v.w));
+}
+// u a(g)
+template <bool kSilu>
+__device__ __forceinline__ f2 gated(f2 u, f2 g) {
+  float a, b;
+  elem::upk(mul(g, pk(-kLog2e, -kLog2e)), a, b);
+  elem::upk(elem::add2(pk(ex2f(a), ex2f(b)), pk(1.f, 1.f)), a, b);
+  if constexpr (kSilu) u = mul(u, g);
+  return mul(u, pk(rcpf(a), rcpf(b)));
+}
+
+// kBatch: rows of a thread, whose loads are in flight together (rows of a head of 128 channels are 16 bytes a lane each).
+template <bool kBlock, int V, bool kWFp32, bool kSilu, bool kFirst, int kBatch>
 __global__ void gated_norm_kernel(const GatedNormParams p, int lanes) {
-  __shared__ float scratch[32];
+  __shared__ float scratch[kBatch][32];
   grid_dependency_wait();
-  const Place at = place<kBlock>(p.rows, lanes);
-  const int64_t token = at.row / p.H;
-  const int h = static_cast<int>(at.row - token * p.H), pieces = p.D / 8;
-  const __nv_bfloat16* x = p.x + at_token(p.xs, token, p.T) + static_cast<int64_t>(h) * p.D;
-  const __nv_bfloat16* g = p.gate + at_token(p.gs, token, p.T) + static_cast<int64_t>(h) * p.D;
-  uint4 xw[V], gw[V];
+  const int pieces = p.D / 8, per = kBlock ? 1 : blockDim.x / lanes;
+  const int lane = kBlock ? threadIdx.x : threadIdx.x % lanes, step = kBlock ? blockDim.x : lanes;
+  uint4 xw[kBatch][V], gw[kBatch][V];
+  unsigned token[kBatch], h[kBatch];
+  bool live[kBatch];
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const int c = at.lane + i * at.lanes;
-    xw[i] = gw[i] = make_uint4(0u, 0u, 0u, 0u);
-    if (c < pieces) {
-      xw[i] = *reinterpret_cast<const uint4*>(x + 8 * c);
-      gw[i] = *reinterpret_cast<const uint4*>(g + 8 * c);
+  for (int r = 0; r < kBatch; ++r) {
+    unsigned row = (blockIdx.x * kBatch + r) * per + (kBlock ? 0 : threadIdx.x / lanes);
+    live[r] = row < p.rows;
+    if (!live[r]) row = static_cast<unsigned>(p.rows) - 1;         // (takes part in the sums, stores nothing)
+    token[r] = row / static_cast<unsigned>(p.H);
+    h[r] = row - token[r] * static_cast<unsigned>(p.H);
+    const __nv_bfloat16* x = p.x + at_token(p.xs, token[r], p.T) + static_cast<int64_t>(h[r]) * p.D;
+    const __nv_bfloat16* g = p.gate + at_token(p.gs, token[r], p.T) + static_cast<int64_t>(h[r]) * p.D;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int c = lane + i * step;
+      xw[r][i] = gw[r][i] = make_uint4(0u, 0u, 0u, 0u);
+      if (c < pieces) {
+        xw[r][i] = *reinterpret_cast<const uint4*>(x + 8 * c);
+        gw[r][i] = *reinterpret_cast<const uint4*>(g + 8 * c);
+      }
     }
   }
-  float u[V][8], sum = 0.f;
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    unpack8(xw[i], u[i]);
-    if constexpr (kFirst) {
-      float a[8];
-      unpack8(gw[i], a);
+  for (int r = 0; r < kBatch; ++r) {
+    f2 u[V][4], sum = pk(0.f, 0.f);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) u[i][e] *= kSilu ? a[e] * sigmoid_exact(a[e]) : sigmoid_exact(a[e]);
+    for (int i = 0; i < V; ++i) {
+      f2 g[4];
+      unpack(xw[r][i], u[i]);
+      unpack(gw[r][i], g);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if constexpr (kFirst) u[i][e] = gated<kSilu>(u[i][e], g[e]);
+        sum = fma2(u[i][e], u[i][e], sum);
+      }
     }
+    float lo, hi;
+    elem::upk(sum, lo, hi);
+    const float root = rsqrtf(row_sum<kBlock>(lo + hi, lanes, scratch[r]) / static_cast<float>(p.D) + p.eps);
+    if (!live[r]) continue;
+    __nv_bfloat16* out = p.out + at_token(p.os, token[r], p.T) + static_cast<int64_t>(h[r]) * p.D;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sum = fmaf(u[i][e], u[i][e], sum);
-  }
-  const float r = rsqrtf(row_sum<kBlock>(sum, lanes, scratch) / static_cast<float>(p.D) + p.eps);
-  if (!at.live) return;
-  __nv_bfloat16* out = p.out + at_token(p.os, token, p.T) + static_cast<int64_t>(h) * p.D;
+    for (int i = 0; i < V; ++i) {
+      const int c = lane + i * step;
+      if (c >= pieces) break;
+      float w[8];
+      load8<kWFp32>(p.weight, (p.per_head ? static_cast<int64_t>(h[r]) * p.D : 0) + 8 * c, w);
+      f2 g[4];
+      unpack(gw[r][i], g);
+      uint32_t o[4];
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const int c = at.lane + i * at.lanes;
-    if (c >= pieces) break;
-    float w[8], a[8];
-    load8<kWFp32>(p.weight, (p.per_head ? static_cast<int64_t>(h) * p.D : 0) + 8 * c, w);
-    if constexpr (!kFirst) unpack8(gw[i], a);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      u[i][e] *= r * w[e];
-      if constexpr (!kFirst) u[i][e] *= kSilu ? a[e] * sigmoid_exact(a[e]) : sigmoid_exact(a[e]);
+      for (int e = 0; e < 4; ++e) {
+        f2 y = mul(u[i][e], mul(pk(root, root), pk(w[2 * e], w[2 * e + 1])));
+        if constexpr (!kFirst) y = gated<kSilu>(y, g[e]);
+        o[e] = elem::round_bf(y);
+      }
+      *reinterpret_cast<uint4*>(out + 8 * c) = make_uint4(o[0], o[1], o[2], o[3]);
     }
-    *reinterpret_cast<uint4*>(out + 8 * c) = pack8(u[i]);
   }
 }
 
@@ -110,8 +149,8 @@ __global__ void add_norm_kernel(const AddNormParams p, int lanes) {
   grid_dependency_wait();
   const Place at = place<kBlock>(p.rows, lanes);
   const int pieces = p.D / 8;
-  const __nv_bfloat16* x = p.x + at_token(p.xs, at.row, p.T);
-  const int64_t from = at_token(p.rs, at.row, p.T);
+  const __nv_bfloat16* x = p.x + at_token(p.xs, static_cast<unsigned>(at.row), p.T);
+  const int64_t from = at_token(p.rs, static_cast<unsigned>(at.row), p.T);
   uint4 xw[V];
   float u[V][8], sum = 0.f;
 #pragma unroll
@@ -131,7 +170,7 @@ __global__ void add_norm_kernel(const AddNormParams p, int lanes) {
       }
     }
   }
-  const int64_t to = at_token(p.ros, at.row, p.T);
+  const int64_t to = at_token(p.ros, static_cast<unsigned>(at.row), p.T);
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const int c = at.lane + i * at.lanes;
@@ -154,7 +193,7 @@ __global__ void add_norm_kernel(const AddNormParams p, int lanes) {
   }
   const float r = rsqrtf(row_sum<kBlock>(sum, lanes, scratch) / static_cast<float>(p.D) + p.eps);
   if (!at.live) return;
-  __nv_bfloat16* out = p.out + at_token(p.os, at.row, p.T);
+  __nv_bfloat16* out = p.out + at_token(p.os, static_cast<unsigned>(at.row), p.T);
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const int c = at.lane + i * at.lanes;
@@ -191,16 +230,26 @@ inline Split split_of(int D) {
   ((s).block ? ((s).v == 2 ? norm::name<true, 2, __VA_ARGS__> : norm::name<true, 4, __VA_ARGS__>)                          \
              : ((s).v == 1 ? norm::name<false, 1, __VA_ARGS__> : (s).v == 2 ? norm::name<false, 2, __VA_ARGS__> : norm::name<false, 4, __VA_ARGS__>))
 
+namespace norm {
+template <bool kWFp32, bool kSilu, bool kFirst>
+void (*pick_gated(const Split& s, bool four))(GatedNormParams, int) {
+  if (four) return gated_norm_kernel<false, 1, kWFp32, kSilu, kFirst, 4>;
+  return FKDA_NORM_PICK(gated_norm_kernel, s, kWFp32, kSilu, kFirst, 1);
+}
+}  // namespace norm
+
 cudaError_t launch_gated_norm(const GatedNormParams& p, bool weight_fp32, bool silu, bool gate_first, cudaStream_t stream) {
   if (p.rows == 0) return cudaSuccess;
   const norm::Split s = norm::split_of(p.D);
-  const int64_t per = s.block ? 1 : s.threads / s.lanes;
+  // Four short rows a thread once there are enough rows for that to leave every SM two thousand threads.
+  const bool four = !s.block && s.v == 1 && p.rows * s.lanes >= 4 * 2048ll * device_sm_count();
+  const int64_t per = s.block ? 1 : s.threads / s.lanes * (four ? 4 : 1);
   const dim3 grid(static_cast<unsigned>((p.rows + per - 1) / per));
   void (*kernel)(GatedNormParams, int);
-  if (weight_fp32) kernel = silu ? (gate_first ? FKDA_NORM_PICK(gated_norm_kernel, s, true, true, true) : FKDA_NORM_PICK(gated_norm_kernel, s, true, true, false))
-                                 : (gate_first ? FKDA_NORM_PICK(gated_norm_kernel, s, true, false, true) : FKDA_NORM_PICK(gated_norm_kernel, s, true, false, false));
-  else kernel = silu ? (gate_first ? FKDA_NORM_PICK(gated_norm_kernel, s, false, true, true) : FKDA_NORM_PICK(gated_norm_kernel, s, false, true, false))
-                     : (gate_first ? FKDA_NORM_PICK(gated_norm_kernel, s, false, false, true) : FKDA_NORM_PICK(gated_norm_kernel, s, false, false, false));
+  if (weight_fp32) kernel = silu ? (gate_first ? norm::pick_gated<true, true, true>(s, four) : norm::pick_gated<true, true, false>(s, four))
+                                 : (gate_first ? norm::pick_gated<true, false, true>(s, four) : norm::pick_gated<true, false, false>(s, four));
+  else kernel = silu ? (gate_first ? norm::pick_gated<false, true, true>(s, four) : norm::pick_gated<false, true, false>(s, four))
+                     : (gate_first ? norm::pick_gated<false, false, true>(s, four) : norm::pick_gated<false, false, false>(s, four));
   return launch_after(kernel, grid, static_cast<unsigned>(s.threads), 0, stream, p, s.lanes);
 }
 
