@@ -2,6 +2,16 @@
 //
 // y[t][c] = act(bias[c] + sum_k w[c][k] x[t - (W-1) + k][c]).  A thread owns four channels (8 bytes) and walks a tile of tokens with
 // the last W-1 inputs in registers, so that every input is read from memory once, but for the W-1 rows before each tile.
+//
+// Bound by memory: a read and a write an element, against some 30 instructions for four (two of them on the special function unit an
+// element).  What is worked on fills 96 registers, so that an SM holds 640 threads, and one group of four rows each on its way in
+// registers was 20 KB an SM, far from enough: 4 x 8192 x 4352 took 121 us.  Rows come by asynchronous copies through shared memory instead,
+// each thread its own, four groups ahead, without a barrier: 92 us on the same tensors over and over, 6.2 TB/s read and written, and 101 on other ones
+// each time.  (Over and over: three groups ahead 94, six 92; fewer registers - 72, seven blocks an SM - cost spills, 100; groups of two rows 106;
+// prefetches into L2 in place of the copies 104.)
+// Packed sequences of 1 to 300 tokens (30 thousand x 2048 with states) take 50 us, 5.1 TB/s: a sequence's start asks memory for its borders, then for
+// its state and its last rows.
+//
 // States: the last W-1 inputs of a sequence.  Only the thread that owns a sequence's first token reads the initial state, and it
 // writes the final one behind that (from the sequence's last rows), so the two may be one tensor; for that it also walks the tokens
 // behind its tile that still see the initial state, which the next tile leaves out.
@@ -18,7 +28,15 @@ using elem::pk;
 
 constexpr int kThreads = 128;
 constexpr int kOwn = 4;            // channels of a thread
-constexpr int kGroup = 4;          // tokens whose loads are in flight together, while those of the group before are worked on
+constexpr int kGroup = 4;          // tokens that are worked on together
+constexpr int kAhead = 4;          // groups on their way meanwhile
+
+__device__ __forceinline__ void cp_async8(uint32_t to, const void* from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kLeft>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory"); }
 
 __device__ __forceinline__ void unpack(const uint2& v, f2 (&x)[2]) {
   x[0] = pk(bf_lo(v.x), bf_hi(v.x));
@@ -33,6 +51,7 @@ __device__ __forceinline__ f2 silu(f2 y) {
 
 template <int W, bool kWFp32, bool kPacked, bool kSilu>
 __global__ void __launch_bounds__(kThreads, 5) conv_kernel(const ConvParams p) {
+  __shared__ uint2 ring[kAhead + 1][kGroup][kThreads];
   grid_dependency_wait();
   const unsigned vecs = static_cast<unsigned>(p.C) / kOwn;
   const int64_t flat = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
@@ -108,7 +127,6 @@ __global__ void __launch_bounds__(kThreads, 5) conv_kernel(const ConvParams p) {
     }
     return make_uint2(elem::round_bf(y[0]), elem::round_bf(y[1]));
   };
-  bool fresh = true;                              // what reaches back has to be loaded
   while (true) {
     if (t >= eos) {
       if constexpr (!kPacked) break;
@@ -123,49 +141,49 @@ __global__ void __launch_bounds__(kThreads, 5) conv_kernel(const ConvParams p) {
       if (bos < t) bos = t;                       // (only where cu_seqlens is not monotone)
       t = bos;
       eos = next;
-      fresh = true;
     }
     const int64_t limit = bos >= t0 && bos + W - 1 > end ? (bos + W - 1 < eos ? bos + W - 1 : eos) : (end < eos ? end : eos);
     if (t >= limit || (bos >= end && t >= end)) break;
-    if (fresh) {
-      fresh = false;
+    const __nv_bfloat16* from = x + t * p.xs.token;
+    __nv_bfloat16* to = out + t * p.os.token;
+    int left = static_cast<int>(limit - t);
+    // groups on the way to shared memory, each thread's own
+    auto ask = [&](int ahead, int slot) {          // (`ahead` groups from `from`)
+      if (left >= (ahead + 1) * kGroup) {
 #pragma unroll
-      for (int j = 0; j < W - 1; ++j) {
-        const int64_t at = t - (W - 1) + j;
-        uint2 v = make_uint2(0u, 0u);
-        if (at >= bos) v = *reinterpret_cast<const uint2*>(x + at * p.xs.token);
-        else if (p.initial_state != nullptr) v = *reinterpret_cast<const uint2*>(p.initial_state + (n * (W - 1) + (W - 1) + at - bos) * p.C + c);
-        unpack(v, u[j]);
+        for (int i = 0; i < kGroup; ++i) cp_async8(smem_u32(&ring[slot][i][threadIdx.x]), from + (ahead * kGroup + i) * p.xs.token);
       }
-      if (t == bos && p.final_state != nullptr) {
-        uint2 last[W - 1];
+      cp_async_commit();
+    };
+    int slot = 0;
 #pragma unroll
-        for (int j = 0; j < W - 1; ++j) {
-          const int64_t at = eos - (W - 1) + j;
-          last[j] = make_uint2(0u, 0u);
-          if (at >= bos) last[j] = *reinterpret_cast<const uint2*>(x + at * p.xs.token);
-          else if (p.initial_state != nullptr) last[j] = *reinterpret_cast<const uint2*>(p.initial_state + (n * (W - 1) + (W - 1) + at - bos) * p.C + c);
-        }
+    for (int g = 0; g < kAhead; ++g) ask(g, g);
+    {
+      auto row_at = [&](int64_t at) {             // (rows before the sequence: of its initial state)
+        if (at >= bos) return *reinterpret_cast<const uint2*>(x + at * p.xs.token);
+        if (p.initial_state != nullptr) return *reinterpret_cast<const uint2*>(p.initial_state + (n * (W - 1) + (W - 1) + at - bos) * p.C + c);
+        return make_uint2(0u, 0u);
+      };
+      const bool leave = t == bos && p.final_state != nullptr;
+      uint2 back[W - 1], last[W - 1];
+#pragma unroll
+      for (int j = 0; j < W - 1; ++j) back[j] = row_at(t - (W - 1) + j);
+      if (leave) {
+#pragma unroll
+        for (int j = 0; j < W - 1; ++j) last[j] = row_at(eos - (W - 1) + j);
 #pragma unroll
         for (int j = 0; j < W - 1; ++j) *reinterpret_cast<uint2*>(p.final_state + (n * (W - 1) + j) * p.C + c) = last[j];
       }
-    }
-    const __nv_bfloat16* from = x + t * p.xs.token;
-    __nv_bfloat16* to = out + t * p.os.token;
-    uint2 in[kGroup];
-    int left = static_cast<int>(limit - t);
-    if (left >= kGroup) {
 #pragma unroll
-      for (int i = 0; i < kGroup; ++i) in[i] = *reinterpret_cast<const uint2*>(from + i * p.xs.token);
+      for (int j = 0; j < W - 1; ++j) unpack(back[j], u[j]);
     }
     for (; left >= kGroup; left -= kGroup) {
+      cp_async_wait<kAhead - 1>();
 #pragma unroll
-      for (int i = 0; i < kGroup; ++i) unpack(in[i], u[W - 1 + i]);
+      for (int i = 0; i < kGroup; ++i) unpack(ring[slot][i][threadIdx.x], u[W - 1 + i]);
+      ask(kAhead, slot == 0 ? kAhead : slot - 1);     // (into the slot of the group before, whose rows are in use no more)
+      slot = slot == kAhead ? 0 : slot + 1;
       from += kGroup * p.xs.token;
-      if (left >= 2 * kGroup) {
-#pragma unroll
-        for (int i = 0; i < kGroup; ++i) in[i] = *reinterpret_cast<const uint2*>(from + i * p.xs.token);
-      }
 #pragma unroll
       for (int i = 0; i < kGroup; ++i) *reinterpret_cast<uint2*>(to + i * p.os.token) = result(i);
       to += kGroup * p.os.token;
@@ -174,15 +192,17 @@ __global__ void __launch_bounds__(kThreads, 5) conv_kernel(const ConvParams p) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) u[j][e] = u[kGroup + j][e];
     }
-    for (; left > 0; --left) {                  // (what is left of a group)
-      unpack(*reinterpret_cast<const uint2*>(from), u[W - 1]);
-      *reinterpret_cast<uint2*>(to) = result(0);
-      from += p.xs.token;
-      to += p.os.token;
+    if (left > 0) {                             // (what is left of a group: nothing follows on it)
+      uint2 in[kGroup - 1];
 #pragma unroll
-      for (int j = 0; j < W - 1; ++j)
+      for (int i = 0; i < kGroup - 1; ++i)
+        if (i < left) in[i] = *reinterpret_cast<const uint2*>(from + i * p.xs.token);
 #pragma unroll
-        for (int e = 0; e < 2; ++e) u[j][e] = u[j + 1][e];
+      for (int i = 0; i < kGroup - 1; ++i) {
+        if (i >= left) break;
+        unpack(in[i], u[W - 1 + i]);
+        *reinterpret_cast<uint2*>(to + i * p.os.token) = result(i);
+      }
     }
     t = limit;
     if (t >= end && t < eos) break;
@@ -207,10 +227,10 @@ cudaError_t launch(const ConvParams& p, bool weight_fp32, cudaStream_t stream) {
 cudaError_t launch_short_conv(ConvParams p, int width, bool weight_fp32, cudaStream_t stream) {
   const bool packed = p.cu_seqlens != nullptr;
   const int64_t vectors = static_cast<int64_t>(packed ? 1 : p.N) * p.T * (p.C / conv::kOwn);
-  // Tokens per thread: as many as leave every SM two thousand threads (the rows before a tile are read again, 3 of 64, and its weights), but no
-  // fewer than the taps that reach back: only a sequence's first tile may see its initial state.
+  // Tokens per thread: as many as leave every SM a thousand threads (the rows before a tile are read again, 3 of 64, and its weights; 128 tokens took
+  // 96 us where 64 take 92), but no fewer than the taps that reach back: only a sequence's first tile may see its initial state.
   int tile = 64;
-  while (tile > 4 && vectors / tile < 2048ll * device_sm_count()) tile >>= 1;
+  while (tile > 4 && vectors / tile < 1024ll * device_sm_count()) tile >>= 1;
   p.tile = !packed && p.T < tile ? static_cast<int>(p.T > 0 ? p.T : 1) : tile;
   p.tiles = static_cast<int>((p.T + p.tile - 1) / p.tile);
   switch (width) {
