@@ -41,7 +41,7 @@ struct SsmScanParams {
   void* final_state;
   const int64_t* cu_seqlens;
   SsmPlan* plan;             // packed batches
-  float* slots;              // [slot][128][Ns] states of runs, slot = run * pairs + pair
+  float4* slots;             // [slot][Ns / 4][128 rows] states of runs, slot = run * pairs + pair
   float* decays;             // [slot][2] decay over a run, per head
   int* status;
   unsigned* queue;           // packed batches: counter that hands the walks out, or nullptr: a CTA each
@@ -51,6 +51,7 @@ struct SsmScanParams {
   int pairs_per_group, pairs;
   int runs, run_blocks;      // equal lengths
   int packed;
+  int late;                  // full pass behind a first one: waits for it where it wants the states, not before
   int state_fp32;
   int wait_limit_us;         // test aids, as in ScanParams
   int stop_loads_after;

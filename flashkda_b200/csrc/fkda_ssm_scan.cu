@@ -205,7 +205,8 @@ __global__ void __launch_bounds__(kThreads, 1) ssm_scan_kernel(const __grid_cons
   }
   uint32_t tmem_base = 0;
   volatile unsigned* next = reinterpret_cast<volatile unsigned*>(smem + L::kMisc + 8);
-  grid_dependency_wait();
+  // Packed batches read their plan to begin with, the others nothing but what the host gave along until they wait further down.
+  if (p.packed) grid_dependency_wait();
   // Packed batches: as many CTAs as there are SMs take one walk after the other, the longest first.
   for (unsigned turn = 0;; ++turn) {
   if (warp == 0) {
@@ -223,13 +224,18 @@ __global__ void __launch_bounds__(kThreads, 1) ssm_scan_kernel(const __grid_cons
   tmem_base = tmem;
   bool ok = *abort_flag <= 0;
   const SsmItem it = ssm_item(p, *next, kFull);
+  // The launches behind this one may begin with what they can do before they wait in their turn.  Of the full pass behind a first one that is
+  // everything but the states: what the caller's kernels wrote was there before the first pass went past its own wait.  (It reads around the
+  // first-level cache.)
+  if (!kFull || !p.late) grid_dependency_wait();
+  if (!kFull) grid_release_next();
   const int blocks = ok ? it.blocks : 0;
   if (warp < 8) {
     if constexpr (kFull) {
       const int q = warp >> 2, w = warp & 3;                          // column blocks q, q + 2; rows 32 w + lane
       const uint32_t lanes = tmem + (static_cast<uint32_t>(32 * w) << 16);
       const bool mine = kWide || q == 0 || it.two;                    // (this warpgroup's half of the output)
-      const float D = blocks > 0 && mine && p.D != nullptr ? __ldg(p.D + it.head0 + (kWide ? 0 : q)) : 0.f;
+      const float D = blocks > 0 && mine && p.D != nullptr ? __ldcg(p.D + it.head0 + (kWide ? 0 : q)) : 0.f;
       for (int c = 0; c < blocks; ++c) {
         const Scalars& s = scal[c % kScals];
         if (!(ok = warp_wait(bar(B_SCAL + c % kScals), (c / kScals) & 1, abort_flag))) break;
@@ -301,7 +307,7 @@ __global__ void __launch_bounds__(kThreads, 1) ssm_scan_kernel(const __grid_cons
     const uint32_t at = tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16) + kColS + g * kOwn;
     const bool there = kWide || h == 0 || it.two;
     const int64_t state = ((static_cast<int64_t>(it.n) * p.H + it.head0 + h) * (kWide ? 128 : 64) + (kWide ? row : row & 63)) * kNs + g * kOwn;
-    float* slot = it.slot >= 0 ? p.slots + (static_cast<int64_t>(it.slot) * 128 + row) * kNs + g * kOwn : nullptr;
+    float4* slot = it.slot >= 0 ? p.slots + static_cast<int64_t>(it.slot) * (128 * kNs / 4) + (g * kOwn / 4) * 128 + row : nullptr;       // (four columns of a row, 128 further on the next four)
     const int t = tid - 8 * 32;
     // X'^T: this warp's 16 rows of 32, 64 tokens at a time.  A transposed 8 x 8 tile of x has two tokens of a channel in a register, as
     // tensor memory wants them (register 2j | 2j + 1: lane t/4 | t/4 + 8, column 4j + t%4).
@@ -356,10 +362,11 @@ __global__ void __launch_bounds__(kThreads, 1) ssm_scan_kernel(const __grid_cons
           tmem_ld32(at + 32 * part, v);
           tmem_wait_ld();
 #pragma unroll
-          for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(slot + 32 * part + 4 * i) = *reinterpret_cast<const uint4*>(v + 4 * i);
+          for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(slot + (8 * part + i) * 128) = *reinterpret_cast<const uint4*>(v + 4 * i);
         }
       }
     } else {
+      if (p.late) grid_dependency_wait();
       if (blocks > 0) {
 #pragma unroll 1
         for (int part = 0; part < kOwn / 32; ++part) {
@@ -367,8 +374,11 @@ __global__ void __launch_bounds__(kThreads, 1) ssm_scan_kernel(const __grid_cons
 #pragma unroll
           for (int i = 0; i < 32; ++i) v[i] = 0u;
           if (there) {
-            if (slot != nullptr || (p.initial_state != nullptr && p.state_fp32)) {
-              const float* src = (slot != nullptr ? slot : static_cast<const float*>(p.initial_state) + state) + 32 * part;
+            if (slot != nullptr) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(v + 4 * i) = *reinterpret_cast<const uint4*>(slot + (8 * part + i) * 128);
+            } else if (p.initial_state != nullptr && p.state_fp32) {
+              const float* src = static_cast<const float*>(p.initial_state) + state + 32 * part;
 #pragma unroll
               for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(v + 4 * i) = *reinterpret_cast<const uint4*>(src + 4 * i);
             } else if (p.initial_state != nullptr) {
@@ -568,15 +578,15 @@ __global__ void __launch_bounds__(kThreads, 1) ssm_scan_kernel(const __grid_cons
     auto load_dt = [&](int c, uint32_t (&to)[4]) {
       const int64_t left = c < mine ? it.tokens - static_cast<int64_t>(kFull ? c : blocks - 1 - c) * kQ - 4 * lane : 0;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) to[k] = k < left ? static_cast<uint32_t>(__ldg(src + k * pitch)) << 16 : 0u;
+      for (int k = 0; k < 4; ++k) to[k] = k < left ? static_cast<uint32_t>(__ldcg(src + k * pitch)) << 16 : 0u;
       src += turn_on;
     };
     uint32_t raw[4], then[4], after_then[4];
     load_dt(0, raw);
     load_dt(1, then);
     if (mine > 0) {
-      A = -kLog2e * ex2f(kLog2e * __ldg(p.A_log + head));
-      bias = __ldg(p.dt_bias + head);
+      A = -kLog2e * ex2f(kLog2e * __ldcg(p.A_log + head));
+      bias = __ldcg(p.dt_bias + head);
     }
 #pragma unroll 1
     for (int c = 0; c < mine; ++c) {
@@ -726,6 +736,7 @@ __global__ void __launch_bounds__(kThreads, 1) ssm_scan_kernel(const __grid_cons
   __syncthreads();
   if (*abort_flag > 0 || p.queue == nullptr || !it.there) break;
   }
+  if (kFull && p.late) grid_dependency_wait();       // (all of it: what follows in the stream waits for this launch alone)
   if (tid == 0 && *abort_flag > 0) atomicCAS(p.status, kStatusOk, kStatusWaitTimeout);
   if (warp == 17) {
     tc_fence_after();
@@ -868,7 +879,8 @@ __global__ void __launch_bounds__(kPlanThreads) ssm_plan_kernel(const int64_t* c
 
 // Per sequence that is cut: its runs' local states -> the state that each run starts from.
 __global__ void __launch_bounds__(256) ssm_chain_kernel(const SsmScanParams p, int Ns, int pairs) {
-  grid_dependency_wait();
+  grid_release_next();
+  if (p.packed) grid_dependency_wait();
   const int pieces = 128 * Ns / 4 / 256;                              // blocks of 256 float4
   const int piece = static_cast<int>(blockIdx.x % pieces), pair = static_cast<int>(blockIdx.x / pieces % pairs);
   const int stride = static_cast<int>(gridDim.x / pieces / pairs), ranks = p.packed ? p.plan->cut : p.N;
@@ -879,20 +891,22 @@ __global__ void __launch_bounds__(256) ssm_chain_kernel(const SsmScanParams p, i
     first = p.plan->slot_prefix(p.N)[rank];
     runs = p.plan->slot_prefix(p.N)[rank + 1] - first;
   }
-  const int at = (piece * 256 + threadIdx.x) * 4, row = at / Ns;
+  const int at = piece * 256 + threadIdx.x, row = at & 127, column = (at >> 7) * 4;      // (the order of the states' memory)
   const int per = p.P == 128 ? 1 : 2, in_group = p.H / p.G, group = pair / p.pairs_per_group;
   const int within = (pair - group * p.pairs_per_group) * per + (per == 2 ? row >> 6 : 0);       // head within its group
   const int h = per == 2 ? row >> 6 : 0;
   float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+  // (the caller's, which was there before the first pass went past its wait)
   if (p.initial_state != nullptr && within < in_group) {
-    const int64_t src = ((static_cast<int64_t>(n) * p.H + group * in_group + within) * p.P + (per == 2 ? row & 63 : row)) * Ns + at % Ns;
+    const int64_t src = ((static_cast<int64_t>(n) * p.H + group * in_group + within) * p.P + (per == 2 ? row & 63 : row)) * Ns + column;
     if (p.state_fp32) {
-      s = *reinterpret_cast<const float4*>(static_cast<const float*>(p.initial_state) + src);
+      s = __ldcg(reinterpret_cast<const float4*>(static_cast<const float*>(p.initial_state) + src));
     } else {
-      const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(p.initial_state) + src);
+      const uint2 w = __ldcg(reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(p.initial_state) + src));
       s = make_float4(bf_lo(w.x), bf_hi(w.x), bf_lo(w.y), bf_hi(w.y));
     }
   }
+  grid_dependency_wait();
   // (eight runs' states and decays on their way at a time: one behind the other, a run takes 1.9 us)
   constexpr int kAhead = 8;
   for (int r0 = 0; r0 < runs; r0 += kAhead) {
@@ -902,7 +916,7 @@ __global__ void __launch_bounds__(256) ssm_chain_kernel(const SsmScanParams p, i
     for (int i = 0; i < kAhead; ++i) {
       const int64_t slot = static_cast<int64_t>(first + r0 + i) * pairs + pair;
       if (r0 + i + 1 < runs) {
-        local[i] = *reinterpret_cast<const float4*>(p.slots + slot * 128 * Ns + at);
+        local[i] = p.slots[slot * (32 * Ns) + at];
         d[i] = p.decays[2 * slot + h];
       }
     }
@@ -910,7 +924,7 @@ __global__ void __launch_bounds__(256) ssm_chain_kernel(const SsmScanParams p, i
     for (int i = 0; i < kAhead; ++i) {
       if (r0 + i >= runs) break;
       const int64_t slot = static_cast<int64_t>(first + r0 + i) * pairs + pair;
-      *reinterpret_cast<float4*>(p.slots + slot * 128 * Ns + at) = s;
+      p.slots[slot * (32 * Ns) + at] = s;
       if (r0 + i + 1 < runs) s = make_float4(fmaf(d[i], s.x, local[i].x), fmaf(d[i], s.y, local[i].y), fmaf(d[i], s.z, local[i].z), fmaf(d[i], s.w, local[i].w));
     }
   }
@@ -1011,7 +1025,7 @@ cudaError_t launch_ssm_scan(const SsmParams& q, const SsmLayout& L, const SsmAid
   p.final_state = q.final_state;
   p.cu_seqlens = q.cu_seqlens;
   p.plan = reinterpret_cast<SsmPlan*>(ws + L.plan_off);
-  p.slots = reinterpret_cast<float*>(ws + L.slot_off);
+  p.slots = reinterpret_cast<float4*>(ws + L.slot_off);
   p.decays = reinterpret_cast<float*>(ws + L.decay_off);
   p.status = reinterpret_cast<int*>(ws);
   p.dts = q.dts;
@@ -1047,6 +1061,7 @@ cudaError_t launch_ssm_scan(const SsmParams& q, const SsmLayout& L, const SsmAid
     if (e != cudaSuccess) return e;
   }
   if (packed) p.queue = p.plan->next + 1;
+  p.late = !packed && L.first_items > 0;
   return ssm_scan::launch_pass<true>(maps, p, q.Ns, L.items, stream);
 }
 
