@@ -7,8 +7,11 @@
 namespace fkda {
 
 constexpr int kSsmBlock = 128;       // tokens of a block
-// Sequences of at most this many tokens go token by token (fkda_ssm_step.cu).
-constexpr int kSsmStepT = 8;
+// Sequences of at most this many tokens go token by token (fkda_ssm_step.cu).  Both sides, us, with fp32 states in and out:
+//     heads, P x Ns, batch      32, 64 x 128, 1    32, 64 x 128, 16    32, 64 x 128, 128    32, 128 x 128, 128    32, 64 x 64, 128
+//     16 tokens one by one / in blocks   6.4 / 12.9          25 / 27            144 / 180             278 / 335              75 / 139
+//     32 tokens                         10.7 / 13.0          42 / 28            260 / 183             505 / 339             133 / 141
+constexpr int kSsmStepT = 16;
 constexpr int kSsmPlanMost = 2048;   // packed batches of more sequences keep the given order and are not cut into runs
 // What the planner of runs reckons with, in hundredths of a block's walk (some 3 us): a block of the first pass, what a walk takes beside its
 // blocks, the launch that chains runs, and (in hundredths of that) what a run's state of a pair of heads takes on its way through memory.

@@ -21,6 +21,21 @@
 // Decays: every exponent that is evaluated is a sum of terms of one sign, so that nothing cancels, but for those within 32 x 32 blocks on
 // the diagonal, which are differences of sums over less than 32 tokens.
 // Rows past a sequence's end are zeroed in the tiles of x and B where they are summed over; those of C only reach outputs that are not stored.
+//
+// What bounds it (4 x 8192 tokens, 32 heads of P = Ns = 128: 128 CTAs of 64 blocks, 208 us on tensors that are new each time, 180 over and over; 572 MB,
+// 2.7 TB/s; 86 GFLOP as 5 P Ns a token).  Not memory: a block takes 4400 to 4900 cycles, of which its tiles would take 2700.  The products take 2560 of
+// them, all on one chain: M X is done, the output is read out of tensor memory (1100 cycles), C S^T goes there (550), X'^T B (1020), M X (700).  G and C S^T
+// read both operands from shared memory at all that it gives, 128 bytes a cycle, and hold up the other warps' accesses meanwhile.  Left out to see: half
+// of G saves 8 us, the lo part 14, as much as their cycles; reads of x for the output 2, the state's copy and the output's rescaling 1.
+// Taken: five products of 128 x 128 x 128 on two heads at once, since one head of P = 64 would leave half of a product's rows empty; X'^T in tensor memory
+// (in shared memory: 281 us); a warp a block of M (a table of masks, one copy of the code: unrolled for each kind of block, the kernel no
+// longer fitted in the instruction caches, 10 %).  Taken back: X'^T B before C S^T (the state's warps then wait for C S^T: 186 for 180, packed 435 for 397),
+// the output on warps 8-15 (236), tiles of B and C asked for in the L2 beforehand (none).
+//
+// Few chains are cut into runs (fkda_ssm.cuh): a first pass leaves what each run adds to a zero state, 1.3 us a block, a small launch chains these, and the
+// full pass starts every run from its state.  One sequence of 131072 x 8 heads of 64 takes 164 us (67 ms token by token; 40 us first pass,
+// 8 chaining, 80 full), a prompt of 777 x 32 heads 19.5 us: there each launch's start counts, some 2.5 us until decays and the first tiles are there, most of it
+// fetching code, so that the launches overlap (see the waits below).  Packed batches of 16 sequences of 256 to 16384 tokens, 32 heads: 434 us, 2.5 TB/s.
 #include "fkda_elem.cuh"
 #include "fkda_layer.cuh"
 #include "fkda_ssm.cuh"

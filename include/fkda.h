@@ -243,7 +243,7 @@ typedef struct fkda_ssm_params {
   uint32_t flags;            /* 0 or FKDA_FLAG_STATUS_UNREAD */
 } fkda_ssm_params;
 /* Bytes of workspace that fkda_ssm_fwd needs for these sizes, on the current device (data pointers other than cu_seqlens are not looked at):
- * 0 for equal lengths of at most 8 tokens.  Its first word is the call's status, as fkda_read_status reads it. */
+ * 0 for equal lengths of at most 16 tokens.  Its first word is the call's status, as fkda_read_status reads it. */
 int fkda_ssm_scratch_bytes(const fkda_ssm_params* p, int64_t* bytes);
 int fkda_ssm_fwd(const fkda_ssm_params* p, void* cuda_stream);
 
