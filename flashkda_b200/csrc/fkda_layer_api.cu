@@ -168,6 +168,8 @@ int check_ssm(const fkda_ssm_params* p) {
   for (const View* v : {&x, &dt, &b, &c, &o})
     if (ranges_meet(p->final_state, states, v->base, span(*v, s))) return set_error(FKDA_ERR_INVALID_ARGUMENT, "final_state shares memory with %s", v->name);
   if (ranges_meet(p->initial_state, states, p->out, span(o, s))) return refuse("out shares memory with initial_state");
+  for (const float* parameter : {p->A_log, p->dt_bias, p->D})
+    if (over(o, s, parameter, p->H, FKDA_STATE_FP32) || ranges_meet(p->final_state, states, parameter, p->H * 4)) return refuse("an output shares memory with A_log, dt_bias or D");
   return FKDA_OK;
 }
 
@@ -236,6 +238,9 @@ int fkda_short_conv(const fkda_conv_params* p, void* cuda_stream) {
   if (ranges_meet(p->final_state, states, p->x, span(x, s)) || ranges_meet(p->final_state, states, p->out, span(o, s)) ||
       ranges_meet(p->initial_state, states, p->out, span(o, s)))
     return refuse("a state shares memory with x or out");
+  const int64_t size = p->weight_dtype == FKDA_STATE_FP32 ? 4 : 2;
+  if (ranges_meet(p->final_state, states, p->weight, p->C * p->width * size) || ranges_meet(p->final_state, states, p->bias, p->C * size))
+    return refuse("final_state shares memory with weight or bias");
   if ((p->B * p->T + p->N) * (p->C / 8) > (int64_t{1} << 37)) return refuse("too many elements for one call");
   fkda::ConvParams q{};
   q.x = static_cast<const __nv_bfloat16*>(p->x);

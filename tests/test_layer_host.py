@@ -44,7 +44,7 @@ def conv(**more):
     (dict(x_token_stride=66, x_batch_stride=2048), "multiples of 16 bytes"), (dict(x_token_stride=56), "rows of x overlap"), (dict(out_batch_stride=64), "rows of out overlap"), (dict(x_token_stride=-64), "out of range"),
     (dict(x_batch_stride=1 << 60), "out of range"), (dict(out=A), "out shares memory with x"), (dict(out=A + 64), "out shares memory with x"), (dict(x_token_stride=128, x_batch_stride=2048, out=A + 64), "shares memory"),
     (dict(initial_state=D, final_state=D + 16), "overlaps initial_state"), (dict(final_state=A), "state shares memory"), (dict(initial_state=C), "state shares memory"), (dict(initial_state=D + 4), "16-byte boundary"),
-    (dict(out=B), "weight or bias"), (dict(bias=C + 16), "weight or bias"), (dict(T=1 << 39, x_batch_stride=1 << 45, out_batch_stride=1 << 45, out=A << 20), "too (many|large)|out of range")])
+    (dict(out=B), "weight or bias"), (dict(bias=C + 16), "weight or bias"), (dict(final_state=B), "weight or bias"), (dict(final_state=D, bias=D + 64), "weight or bias"), (dict(T=1 << 39, x_batch_stride=1 << 45, out_batch_stride=1 << 45, out=A << 20), "too (many|large)|out of range")])
 def test_short_conv_refusals(more, match):
     refused("fkda_short_conv", conv(**more), match)
 
@@ -61,7 +61,7 @@ def ssm(**more):
     (dict(A_log=None), "A_log"), (dict(dt_bias=None), "dt_bias"), (dict(P=96), "P and the columns"), (dict(Ns=32), "P and the columns"), (dict(G=3), "multiple of G"), (dict(G=0), "multiple of G"),
     (dict(H=0), "H must lie"), (dict(H=70000, G=1), "H must lie"), (dict(N=1), "N must equal B"), (dict(initial_state=0x100000000), "state_dtype"), (dict(cu_seqlens=E), "B must be 1"),
     (dict(x=A + 8), "x must start"), (dict(Bm=C + 8), "B must start"), (dict(C_token_stride=260, C_batch_stride=1 << 17), "multiples of 16 bytes"), (dict(dt_token_stride=3), "rows of dt overlap"), (dict(out_token_stride=128), "rows of out overlap"),
-    (dict(out=A), "out shares memory with x"), (dict(out=C), "out shares memory with B"), (dict(state_dtype=FP32, final_state=A), "final_state shares memory with x"),
+    (dict(out=A), "out shares memory with x"), (dict(out=C), "out shares memory with B"), (dict(D=D + 1024), "shares memory with A_log"), (dict(dt_bias=D + 64), "shares memory with A_log"), (dict(state_dtype=FP32, final_state=E), "shares memory with A_log"), (dict(state_dtype=FP32, final_state=A), "final_state shares memory with x"),
     (dict(state_dtype=FP32, initial_state=D), "out shares memory with initial_state"), (dict(state_dtype=FP32, initial_state=0x100000000, final_state=0x100000010), "overlaps initial_state"),
     (dict(workspace=None), "workspace must be"), (dict(workspace=G + 16), "workspace must be"), (dict(T=1 << 33, x_batch_stride=1 << 41, out_batch_stride=1 << 41), "too many tokens")])
 def test_ssm_refusals(more, match):
