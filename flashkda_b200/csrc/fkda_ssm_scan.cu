@@ -195,6 +195,39 @@ __device__ __noinline__ void make_m(uint32_t at, const Scalars& s, int b, int w,
   }
 }
 
+// 32 rows of the state, half of the columns, from tensor memory to `dst` (its first row).  By way of 32 rows of shared memory (tiles of B and C, free by
+// then): 16 bytes a lane straight from a row each kept the output's warps from shared memory for 2 us.
+template <int kNs, bool kFp32>
+__device__ __noinline__ void leave_state(uint32_t at, uint32_t rows, void* dst) {
+  constexpr int kOwn = kNs / 2, kSize = kFp32 ? 4 : 2, kPieces = kOwn * kSize / 16, kPitch = kOwn * 4;
+  const int lane = threadIdx.x & 31;
+#pragma unroll 1
+  for (int part = 0; part < kOwn / 32; ++part) {
+    uint32_t v[32];
+    tmem_ld32(at + 32 * part, v);
+    tmem_wait_ld();
+#pragma unroll
+    for (int i = 0; i < 2 * kSize; ++i) {
+      const uint32_t to = rows + lane * kPitch + (((2 * kSize * part + i) ^ (lane & 7)) << 4);
+      if constexpr (kFp32) {
+        sts128(to, v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+      } else {
+        uint32_t word[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) word[k] = pack_bf16(__uint_as_float(v[8 * i + 2 * k]), __uint_as_float(v[8 * i + 2 * k + 1]));
+        sts128(to, word[0], word[1], word[2], word[3]);
+      }
+    }
+  }
+  __syncwarp();
+#pragma unroll 4
+  for (int i = lane; i < 32 * kPieces; i += 32) {
+    const int row = i / kPieces, piece = i % kPieces;
+    *reinterpret_cast<uint4*>(static_cast<char*>(dst) + row * (kNs * kSize) + 16 * piece) = lds128(rows + row * kPitch + ((piece ^ (row & 7)) << 4));
+  }
+  fence_proxy_async_smem();                       // (tensor copies write there next)
+}
+
 // kWide: one head of P = 128, else two of P = 64.  kFull: the outputs too, else only what a run adds to a zero state.
 template <int kNs, bool kWide, bool kFull>
 __global__ void __launch_bounds__(kThreads, 1) ssm_scan_kernel(const __grid_constant__ SsmMaps maps, const SsmScanParams p) {
@@ -321,7 +354,7 @@ __global__ void __launch_bounds__(kThreads, 1) ssm_scan_kernel(const __grid_cons
     constexpr int kOwn = kNs / 2;                                     // columns g * kOwn ..
     const uint32_t at = tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16) + kColS + g * kOwn;
     const bool there = kWide || h == 0 || it.two;
-    const int64_t state = ((static_cast<int64_t>(it.n) * p.H + it.head0 + h) * (kWide ? 128 : 64) + (kWide ? row : row & 63)) * kNs + g * kOwn;
+    auto state_at = [&](int r) { return ((static_cast<int64_t>(it.n) * p.H + it.head0 + h) * (kWide ? 128 : 64) + (kWide ? r : r & 63)) * kNs + g * kOwn; };
     float4* slot = it.slot >= 0 ? p.slots + static_cast<int64_t>(it.slot) * (128 * kNs / 4) + (g * kOwn / 4) * 128 + row : nullptr;       // (four columns of a row, 128 further on the next four)
     const int t = tid - 8 * 32;
     // X'^T: this warp's 16 rows of 32, 64 tokens at a time.  A transposed 8 x 8 tile of x has two tokens of a channel in a register, as
@@ -393,11 +426,11 @@ __global__ void __launch_bounds__(kThreads, 1) ssm_scan_kernel(const __grid_cons
 #pragma unroll
               for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(v + 4 * i) = *reinterpret_cast<const uint4*>(slot + (8 * part + i) * 128);
             } else if (p.initial_state != nullptr && p.state_fp32) {
-              const float* src = static_cast<const float*>(p.initial_state) + state + 32 * part;
+              const float* src = static_cast<const float*>(p.initial_state) + state_at(row) + 32 * part;
 #pragma unroll
               for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(v + 4 * i) = *reinterpret_cast<const uint4*>(src + 4 * i);
             } else if (p.initial_state != nullptr) {
-              const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(p.initial_state) + state + 32 * part;
+              const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(p.initial_state) + state_at(row) + 32 * part;
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 const uint4 b = *reinterpret_cast<const uint4*>(src + 8 * i);
@@ -414,90 +447,75 @@ __global__ void __launch_bounds__(kThreads, 1) ssm_scan_kernel(const __grid_cons
         }
         tmem_wait_st();
       }
-      for (int c = 0; blocks > 0 && c <= blocks; ++c) {
-        float d = 1.f;
+      for (int c = 0; c < blocks; ++c) {
         if (c > 0) {
           if (!(ok = warp_wait(bar(B_S_FULL), (c - 1) & 1, abort_flag))) break;
           tc_fence_after();
         }
         const Scalars& s = scal[c % kScals];
-        if (c < blocks) {
-          if (!(ok = warp_wait(bar(B_SCAL + c % kScals), (c / kScals) & 1, abort_flag))) break;
-          d = s.decay[h];
-        }
+        if (!(ok = warp_wait(bar(B_SCAL + c % kScals), (c / kScals) & 1, abort_flag))) break;
+        const float d = s.decay[h];
 #pragma unroll 1
         for (int part = 0; part < kOwn / 32; ++part) {
           uint32_t v[32];
           tmem_ld32(at + 32 * part, v);
           tmem_wait_ld();
-          uint32_t word[16];                                            // as bf16
+          // the copy for C S^T (that of the block before has been read: its product came before those of the state)
+          const uint32_t dst = sbase + L::kS + row * 128;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) word[i] = pack_bf16(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
-          if (c < blocks) {
-            if constexpr (kFull) {
-              // the copy for C S^T (that of the block before has been read: its product came before those of the state)
-              const uint32_t dst = sbase + L::kS + row * 128;
+          for (int i = 0; i < 4; ++i) {
+            const int piece = g * (kOwn / 8) + 4 * part + i;
+            uint32_t word[4];
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int piece = g * (kOwn / 8) + 4 * part + i;
-                sts128(dst + (piece >> 3) * 16384 + (((piece & 7) ^ (row & 7)) << 4), word[4 * i], word[4 * i + 1], word[4 * i + 2], word[4 * i + 3]);
-              }
-            }
-#pragma unroll
-            for (int i = 0; i < 16; ++i) mul2(v[2 * i], v[2 * i + 1], make_float2(d, d));
-            tmem_st32(at + 32 * part, v);
-          } else if (there && it.last && p.final_state != nullptr) {
-            if (p.state_fp32) {
-              float* dst = static_cast<float*>(p.final_state) + state + 32 * part;
-#pragma unroll
-              for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(dst + 4 * i) = *reinterpret_cast<const uint4*>(v + 4 * i);
-            } else {
-              __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.final_state) + state + 32 * part;
-#pragma unroll
-              for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(dst + 8 * i) = make_uint4(word[4 * i], word[4 * i + 1], word[4 * i + 2], word[4 * i + 3]);
-            }
+            for (int k = 0; k < 4; ++k) word[k] = pack_bf16(__uint_as_float(v[8 * i + 2 * k]), __uint_as_float(v[8 * i + 2 * k + 1]));
+            sts128(dst + (piece >> 3) * 16384 + (((piece & 7) ^ (row & 7)) << 4), word[0], word[1], word[2], word[3]);
           }
+#pragma unroll
+          for (int i = 0; i < 16; ++i) mul2(v[2 * i], v[2 * i + 1], make_float2(d, d));
+          tmem_st32(at + 32 * part, v);
         }
-        if (c < blocks) {
-          tmem_wait_st();
-          tc_fence_before();
+        tmem_wait_st();
+        tc_fence_before();
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(B_S_READY));
+
+        if (!(ok = warp_wait(bar(B_FULL_X + c % kXs), (c / kXs) & 1, abort_flag))) break;
+        const uint32_t x = sbase + L::kX + (c % kXs) * kTileX;
+        const int64_t left = it.tokens - static_cast<int64_t>(c) * kQ;
+        if (left < kQ) {
+          // the last block: rows past the end, in the tiles whose rows are summed over
+          if (!(ok = warp_wait(bar(B_FULL_B), c & 1, abort_flag))) break;
+          const uint32_t b = sbase + L::kB;
+          for (int i = t; i < (kQ - static_cast<int>(left)) * 8; i += 256) {
+            const uint32_t off = (static_cast<uint32_t>(left) + i / 8) * 128 + (i % 8) * 16;
+            sts128(x + off, 0u, 0u, 0u, 0u);
+            sts128(x + kTileX / 2 + off, 0u, 0u, 0u, 0u);
+            sts128(b + off, 0u, 0u, 0u, 0u);
+            if (kNs == 128) sts128(b + L::kTile / 2 + off, 0u, 0u, 0u, 0u);
+          }
           fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0) mbar_arrive(bar(B_S_READY));
-
-          if (!(ok = warp_wait(bar(B_FULL_X + c % kXs), (c / kXs) & 1, abort_flag))) break;
-          const uint32_t x = sbase + L::kX + (c % kXs) * kTileX;
-          const int64_t left = it.tokens - static_cast<int64_t>(c) * kQ;
-          if (kFull && left < kQ) {
-            // the last block: rows past the end, in the tiles whose rows are summed over
-            if (!(ok = warp_wait(bar(B_FULL_B), c & 1, abort_flag))) break;
-            const uint32_t b = sbase + L::kB;
-            for (int i = t; i < (kQ - static_cast<int>(left)) * 8; i += 256) {
-              const uint32_t off = (static_cast<uint32_t>(left) + i / 8) * 128 + (i % 8) * 16;
-              sts128(x + off, 0u, 0u, 0u, 0u);
-              sts128(x + kTileX / 2 + off, 0u, 0u, 0u, 0u);
-              sts128(b + off, 0u, 0u, 0u, 0u);
-              if (kNs == 128) sts128(b + L::kTile / 2 + off, 0u, 0u, 0u, 0u);
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar(B_MEET));
-            if (!(ok = warp_wait(bar(B_MEET), 0, abort_flag))) break;
-          }
-          weigh(x, s, kColX, B_XT);
-          if constexpr (kFull) {
-            if (!(ok = warp_wait(bar(B_G), c & 1, abort_flag))) break;
-            tc_fence_after();
-            make_m<kWide>(tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16) + kColG, s, 2 + g, warp & 3, smem + L::kMask);
-            tmem_wait_st();
-            tc_fence_before();
-            __syncwarp();
-          }
-          if (lane == 0) {
-            mbar_arrive(bar(B_SCAL_FREE + c % kScals));
-            mbar_arrive(bar(B_M));
-          }
+          if (lane == 0) mbar_arrive(bar(B_MEET));
+          if (!(ok = warp_wait(bar(B_MEET), 0, abort_flag))) break;
         }
+        weigh(x, s, kColX, B_XT);
+        if (!(ok = warp_wait(bar(B_G), c & 1, abort_flag))) break;
+        tc_fence_after();
+        make_m<kWide>(tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16) + kColG, s, 2 + g, warp & 3, smem + L::kMask);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(bar(B_SCAL_FREE + c % kScals));
+          mbar_arrive(bar(B_M));
+        }
+      }
+      if (ok && blocks > 0 && (ok = warp_wait(bar(B_S_FULL), (blocks - 1) & 1, abort_flag)) && there && it.last && p.final_state != nullptr) {
+        tc_fence_after();
+        const int64_t first = state_at(row - lane);
+        if (p.state_fp32) leave_state<kNs, true>(at, sbase + L::kB + (t - lane) * (kOwn * 4), static_cast<float*>(p.final_state) + first);
+        else leave_state<kNs, false>(at, sbase + L::kB + (t - lane) * (kOwn * 4), static_cast<__nv_bfloat16*>(p.final_state) + first);
       }
     }
   } else if (warp == 17) {
