@@ -106,6 +106,7 @@ __device__ __noinline__ bool wait_on(uint32_t bar, uint32_t parity, volatile int
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
   return __all_sync(0xffffffffu, mbar_try_wait(bar, parity)) || wait_on(bar, parity, abort_flag);
 }
+__device__ __forceinline__ void prefetch_l2(const void* at) { asm volatile("prefetch.global.L2 [%0];" ::"l"(at) : "memory"); }
 __device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
@@ -253,8 +254,37 @@ __global__ void __launch_bounds__(kThreads, 1) ssm_scan_kernel(const __grid_cons
   }
   uint32_t tmem_base = 0;
   volatile unsigned* next = reinterpret_cast<volatile unsigned*>(smem + L::kMisc + 8);
-  // Packed batches read their plan to begin with, the others nothing but what the host gave along until they wait further down.
-  if (p.packed) grid_dependency_wait();
+  // Packed batches read their plan to begin with.  The others know their walk, and ask for what its first block needs while barriers and tensor memory are
+  // set up.  Of the full pass behind a first one that is everything but the states: what the caller's kernels wrote was there before the first pass
+  // went past its own wait.  (It reads around the first-level cache.)
+  if (p.packed) {
+    grid_dependency_wait();
+  } else if (warp == 8 || warp == 16 || warp >= 18) {
+    const SsmItem it = ssm_item(p, blockIdx.x, kFull);
+    if (!kFull || !p.late) grid_dependency_wait();
+    const int64_t start = kFull || it.blocks == 0 ? it.t0 : it.t0 + static_cast<int64_t>(it.blocks - 1) * kQ;
+    const int64_t left = it.t0 + it.tokens - start;
+    if (warp == 19) {
+      if (lane == 0) {
+#pragma unroll
+        for (int i = 0; i < kNs / 64; ++i) {
+          tma_prefetch_3d(&maps.b, it.group * kNs + 64 * i, static_cast<int>(start), static_cast<int>(it.b));
+          if (kFull) tma_prefetch_3d(&maps.c, it.group * kNs + 64 * i, static_cast<int>(start), static_cast<int>(it.b));
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) tma_prefetch_3d(&maps.x, it.head0 * (kWide ? 128 : 64) + 64 * i, static_cast<int>(start), static_cast<int>(it.b));
+      }
+    } else if (warp >= 16) {
+      const __nv_bfloat16* dt = p.dt + it.b * p.dts.batch + (start + 2 * lane + (warp == 18)) * p.dts.token + it.head0;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (2 * lane + (warp == 18) + 64 * i < left) prefetch_l2(dt + 64 * i * p.dts.token);
+      if (lane == 0) prefetch_l2(warp == 18 ? p.A_log + it.head0 : p.dt_bias + it.head0);
+    } else if (kFull && warp == 8 && lane == 0 && p.initial_state != nullptr && it.slot < 0) {
+      const int size = kNs * (p.state_fp32 ? 4 : 2), P = kWide ? 128 : 64;
+      bulk_prefetch_l2(static_cast<const char*>(p.initial_state) + (static_cast<int64_t>(it.n) * p.H + it.head0) * P * size, (kWide || it.two ? 128 : 64) * size);
+    }
+  }
   // Packed batches: as many CTAs as there are SMs take one walk after the other, the longest first.
   for (unsigned turn = 0;; ++turn) {
   if (warp == 0) {
@@ -272,11 +302,8 @@ __global__ void __launch_bounds__(kThreads, 1) ssm_scan_kernel(const __grid_cons
   tmem_base = tmem;
   bool ok = *abort_flag <= 0;
   const SsmItem it = ssm_item(p, *next, kFull);
-  // The launches behind this one may begin with what they can do before they wait in their turn.  Of the full pass behind a first one that is
-  // everything but the states: what the caller's kernels wrote was there before the first pass went past its own wait.  (It reads around the
-  // first-level cache.)
   if (!kFull || !p.late) grid_dependency_wait();
-  if (!kFull) grid_release_next();
+  if (!kFull) grid_release_next();                  // (the launches behind this one wait in their turn)
   const int blocks = ok ? it.blocks : 0;
   if (warp < 8) {
     if constexpr (kFull) {
