@@ -164,6 +164,42 @@ def test_two_streams_at_once():
         assert all(torch.equal(o, case[8]) and torch.equal(f, case[9]) for o, f in outs[s])
 
 
+@pytest.mark.parametrize("captured", [False, True])
+@pytest.mark.parametrize("T,P", [(1500, 64), (700, 128), (20, 64)])
+def test_inputs_that_the_kernel_before_wrote(T, P, captured):
+    """Launches of a scan that is cut into runs overlap: none may read an input before the kernel that writes it, or leave an output to the one behind it too early."""
+    layer = ScanLayer(1, H=2, P=P, seed=T)
+    projs = [randn(1, T, layer.width(), seed=11 + i) for i in range(2)]
+    proj, buf, residual = torch.empty_like(projs[0]), layer.buffers(1, T), torch.empty(1, T, layer.H * P, device="cuda")
+
+    def run():
+        layer.conv_state.zero_()
+        layer.ssm_state.zero_()
+        residual.zero_()
+        layer(proj, residual, buf)
+
+    want = []
+    for q in projs:
+        proj.copy_(q)
+        torch.cuda.synchronize()
+        run()
+        torch.cuda.synchronize()
+        want.append([buf["out"].clone(), residual.clone(), layer.conv_state.clone(), layer.ssm_state.clone()])
+    if captured:
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            run()
+    got = []
+    for i in range(12):
+        proj.copy_(projs[i & 1])
+        graph.replay() if captured else run()
+        got.append([buf["out"].clone(), residual.clone(), layer.conv_state.clone(), layer.ssm_state.clone()])
+    for i, result in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(result, want[i & 1]))
+
+
 def test_the_python_checks_launch_the_same_calls(monkeypatch):
     layer = ScanLayer(2)
     proj, buf = randn(2, 40, layer.width(), seed=3), layer.buffers(2, 40)
