@@ -296,6 +296,7 @@ __global__ void __launch_bounds__(kThreads, 1) ssm_scan_kernel(const __grid_cons
     fence_mbar_init();
   }
   tc_fence_before();
+  __syncwarp();                                     // (every warp comes here as one: lane 0 of most has just been on its own)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
@@ -793,6 +794,7 @@ __global__ void __launch_bounds__(kThreads, 1) ssm_scan_kernel(const __grid_cons
   }
   if (!ok) *abort_flag = 1;
   tc_fence_before();
+  __syncwarp();
   __syncthreads();
   if (*abort_flag > 0 || p.queue == nullptr || !it.there) break;
   }

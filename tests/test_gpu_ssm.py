@@ -114,6 +114,28 @@ def test_packed(lens, H, P, G, Ns, state, surplus):
         assert torch.equal(x0, fin)
 
 
+@pytest.mark.parametrize("P,Ns,H,G", [(64, 128, 32, 1), (64, 64, 19, 1), (128, 128, 16, 2)])
+def test_more_walks_than_multiprocessors(P, Ns, H, G):
+    """Each CTA takes one walk after the other, of different lengths: what a sequence gives alone, within the roundings of both (it may be cut into other runs)."""
+    lens = [int(v) for v in torch.randint(17, 1500, (30,), generator=torch.Generator().manual_seed(P + Ns))]
+    N, T = len(lens), sum(lens)
+    cu = torch.tensor([0] + torch.tensor(lens).cumsum(0).tolist(), device="cuda")
+    x, dt, Bm, Cm, A_log, dt_bias, D, x0 = inputs(1, T, H, P, G, Ns, seed=5, state="fp32", N=N)
+    results = []
+    for _ in range(3):
+        out, fin = torch.full_like(x, float("nan")), torch.full_like(x0, float("nan"))
+        F.ssm_fwd(x, dt, Bm, Cm, out, A_log, dt_bias, D, initial_state=x0, final_state=fin, cu_seqlens=cu)
+        results.append((out, fin))
+    assert all(torch.equal(o, results[0][0]) and torch.equal(f, results[0][1]) for o, f in results)
+    for n in range(0, N, 3):
+        a, b = int(cu[n]), int(cu[n + 1])
+        alone, last = torch.empty_like(x[:, a:b]), torch.empty_like(x0[n:n + 1])
+        F.ssm_fwd(x[:, a:b], dt[:, a:b], Bm[:, a:b], Cm[:, a:b], alone, A_log, dt_bias, D, initial_state=x0[n:n + 1].contiguous(), final_state=last)
+        # each is off by three roundings of its operands and result to bf16 at most (their norms), states by three of 2^-16
+        assert ((out[:, a:b].double() - alone.double()).norm() / alone.double().norm()).item() <= 2 * 3 * R.BF16
+        assert ((fin[n] - last[0]).double().norm() / last.double().norm()).item() <= 2 * 3 * 2.0 ** -16 + 2.0 ** -16
+
+
 def test_no_tokens_hands_the_state_on():
     x, dt, Bm, Cm, A_log, dt_bias, D, x0 = inputs(2, 0, 4, 64, 1, 128, state="fp32")
     fin = torch.empty_like(x0)
