@@ -24,7 +24,8 @@ struct SsmPlan {
   int active;                // sequences that are walked in blocks
   int cut;
   unsigned next[2];          // walks handed out so far: first pass, second pass
-  int pad[3];
+  int walks[2];              // how many there are, of a pair of heads (the first pass's with the last run of each, which it leaves out)
+  int pad;
   __host__ __device__ int* order() { return reinterpret_cast<int*>(this + 1); }
   __host__ __device__ int* prefix(int N) { return order() + N; }
   __host__ __device__ int* slot_prefix(int N) { return prefix(N) + N + 1; }
@@ -60,7 +61,7 @@ struct SsmScanParams {
   int stop_loads_after;
 };
 
-// One CTA's walk.
+// One CTA's walk (packed batches: called by whole warps).
 struct SsmItem {
   bool there;                // false: no more walks
   int n, group, head0;
@@ -83,12 +84,14 @@ __device__ __forceinline__ SsmItem ssm_item(const SsmScanParams& p, unsigned ind
     // (the runs of the first pass are those of the cut sequences, but each one's last: counted with the slots)
     const int* prefix = full ? plan->prefix(p.N) : plan->slot_prefix(p.N);
     const int ranks = full ? plan->active : plan->cut;
-    if (ranks == 0 || rs >= prefix[ranks]) return it;
+    if (rs >= plan->walks[full ? 1 : 0]) return it;
     it.there = true;
+    // (by the whole warp, 32 entries at a time: what one load waits for behind the other is what a walk waits for to begin)
     int lo = 0, hi = ranks;
     while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (prefix[mid] <= rs) lo = mid; else hi = mid;
+      const int step = (hi - lo + 31) >> 5, at = lo + (static_cast<int>(threadIdx.x & 31) + 1) * step;
+      lo += __popc(__ballot_sync(0xffffffffu, at < hi && prefix[at] <= rs)) * step;
+      if (lo + step < hi) hi = lo + step;
     }
     run = rs - prefix[lo];
     runs = prefix[lo + 1] - prefix[lo];

@@ -936,6 +936,8 @@ __global__ void __launch_bounds__(kPlanThreads) ssm_plan_kernel(const int64_t* c
   if (tid == 0) {
     prefix[0] = slots[0] = 0;
     plan->cut = s_cut;
+    plan->walks[0] = done[1];
+    plan->walks[1] = done[0];
   }
 }
 
