@@ -34,8 +34,8 @@
 //
 // Few chains are cut into runs (fkda_ssm.cuh): a first pass leaves what each run adds to a zero state, 1.3 us a block, a small launch chains these, and the
 // full pass starts every run from its state.  One sequence of 131072 x 8 heads of 64 takes 164 us (67 ms token by token; 40 us first pass,
-// 8 chaining, 80 full), a prompt of 777 x 32 heads 19.5 us: there each launch's start counts, some 2.5 us until decays and the first tiles are there, most of it
-// fetching code, so that the launches overlap (see the waits below).  Packed batches of 16 sequences of 256 to 16384 tokens, 32 heads: 434 us, 2.5 TB/s.
+// 8 chaining, 80 full), a prompt of 777 x 32 heads 19.5 us: there each launch's start counts, some 2.5 us until decays and the first tiles are there,
+// so that the launches overlap (see the waits below).  Packed batches of 16 sequences of 256 to 16384 tokens, 32 heads: 434 us, 2.5 TB/s.
 #include "fkda_elem.cuh"
 #include "fkda_layer.cuh"
 #include "fkda_ssm.cuh"
