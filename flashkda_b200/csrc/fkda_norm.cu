@@ -69,14 +69,15 @@ __device__ __forceinline__ void unpack(const uint4& v, f2 (&x)[4]) {
   x[2] = pk(bf_lo(v.z), bf_hi(v.z));
   x[3] = pk(bf_lo(v.w), bf_hi(v.w));
 }
-// u a(g)
+// u a(g).  (a first: where it is 0, u g may be beyond the largest number already)
 template <bool kSilu>
 __device__ __forceinline__ f2 gated(f2 u, f2 g) {
   float a, b;
   elem::upk(mul(g, pk(-kLog2e, -kLog2e)), a, b);
   elem::upk(elem::add2(pk(ex2f(a), ex2f(b)), pk(1.f, 1.f)), a, b);
-  if constexpr (kSilu) u = mul(u, g);
-  return mul(u, pk(rcpf(a), rcpf(b)));
+  f2 act = pk(rcpf(a), rcpf(b));
+  if constexpr (kSilu) act = mul(act, g);
+  return mul(u, act);
 }
 
 // kBatch: rows of a thread, whose loads are in flight together (rows of a head of 128 channels are 16 bytes a lane each).
