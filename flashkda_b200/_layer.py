@@ -201,8 +201,9 @@ def ssm_fwd(x, dt, B, C, out, A_log, dt_bias, D=None, initial_state=None, final_
     bf16 or fp32 [N, H, P, Ns] (same dtype when both are given) or None; they may be one tensor.  cu_seqlens: int64 [N+1] on the device,
     requires B == 1.  A decode step is the call with T == 1.  `out` may not share memory with an input.
 
-    `workspace` (optional): a uint8 CUDA tensor of at least `ssm_workspace_size(...)` bytes for callers that must not allocate; by default
-    scratch memory comes from torch's caching allocator, where a call needs any."""
+    `workspace` (optional): a uint8 CUDA tensor of at least `ssm_workspace_size(...)` bytes, 256-byte aligned, for callers that must not allocate; by default
+    scratch memory comes from torch's caching allocator, where a call needs any.  `read_status(workspace)` then has the call's status, also of calls that
+    need no scratch memory, if the tensor has at least four bytes."""
     if workspace is None and _handled(_native("ssm_fwd")(x, dt, B, C, out, A_log, dt_bias, D, initial_state, final_state, cu_seqlens)):
         return None
     p = _ssm_params(x, dt, B, C, out, A_log, dt_bias, D, initial_state, final_state, cu_seqlens)

@@ -44,8 +44,8 @@ struct SsmParams {
   int H, P, G, Ns, N;
   int state_fp32;
 };
-// `most`: packed batches, only sequences of at most so many tokens (0: all).
-cudaError_t launch_ssm_step(const SsmParams& p, int most, cudaStream_t stream);
+// `most`: packed batches, only sequences of at most so many tokens (0: all).  `status`: the call's status word, or NULL: not written.
+cudaError_t launch_ssm_step(const SsmParams& p, int most, int* status, cudaStream_t stream);
 
 struct GatedNormParams {
   const __nv_bfloat16* x;

@@ -202,12 +202,16 @@ int do_ssm(const fkda_ssm_params* p, const fkda::SsmAid& aid, void* cuda_stream)
   q.state_fp32 = p->state_dtype == FKDA_STATE_FP32;
   cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
   cudaError_t e;
+  const bool word = p->workspace != nullptr && p->workspace_bytes >= static_cast<int64_t>(sizeof(int)), misplaced = (reinterpret_cast<uintptr_t>(p->workspace) & 255u) != 0;
   if (by_token(p)) {
-    e = fkda::launch_ssm_step(q, 0, stream);
+    // (no scratch memory is needed; one that is given has the status word all the same)
+    const bool told = word && !(p->flags & FKDA_FLAG_STATUS_UNREAD);
+    if (told && misplaced) return refuse("workspace must be 256-byte aligned");
+    e = fkda::launch_ssm_step(q, 0, told ? static_cast<int*>(p->workspace) : nullptr, stream);
     return e == cudaSuccess ? FKDA_OK : cuda_error(e, "selective scan launch");
   }
   const fkda::SsmLayout L = layout_of(p);
-  if (!p->workspace || (reinterpret_cast<uintptr_t>(p->workspace) & 255u)) return refuse("workspace must be non-NULL and 256-byte aligned");
+  if (!p->workspace || misplaced) return refuse("workspace must be non-NULL and 256-byte aligned");
   if (p->workspace_bytes < L.bytes)
     return set_error(FKDA_ERR_WORKSPACE_TOO_SMALL, "workspace has %lld bytes, %lld needed", (long long)p->workspace_bytes, (long long)L.bytes);
   e = fkda::launch_ssm_scan(q, L, aid, p->workspace, !(p->flags & FKDA_FLAG_STATUS_UNREAD), stream);

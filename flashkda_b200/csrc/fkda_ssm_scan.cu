@@ -1111,7 +1111,7 @@ cudaError_t launch_ssm_scan(const SsmParams& q, const SsmLayout& L, const SsmAid
   if (packed) {
     e = launch_after(ssm_scan::ssm_plan_kernel, dim3(1), ssm_scan::kPlanThreads, 0, stream, q.cu_seqlens, q.N, q.T, L.pairs, device_sm_count(), L.least, p.plan, p.status);
     // the sequences of a few tokens, decode steps among the prompts
-    if (e == cudaSuccess) e = launch_ssm_step(q, kSsmStepT, stream);
+    if (e == cudaSuccess) e = launch_ssm_step(q, kSsmStepT, nullptr, stream);
   } else if (clear_status) {
     e = cudaMemsetAsync(ws, 0, 4, stream);
   }

@@ -22,9 +22,17 @@ using elem::pk;
 constexpr int kThreads = 128;
 
 template <int kNs, bool kFp32, bool kPacked>
-__global__ void __launch_bounds__(kThreads) ssm_step_kernel(const SsmParams p, int most) {
+__global__ void __launch_bounds__(kThreads) ssm_step_kernel(const SsmParams p, int most, int* status) {
   constexpr int kLanes = kNs / 8, kRows = 4 * (32 / kLanes) * (kThreads / 32);
   grid_dependency_wait();
+  if (status != nullptr && blockIdx.x == 0) {
+    // (the call's status word: one block looks at all borders, so that the word is written once and no launch has to clear it before)
+    int bad = 0;
+    if constexpr (kPacked)
+      for (int i = threadIdx.x; i < p.N; i += kThreads) bad |= p.cu_seqlens[i] < 0 || p.cu_seqlens[i + 1] < p.cu_seqlens[i] || p.cu_seqlens[i + 1] > p.T;
+    bad = __syncthreads_or(bad);
+    if (threadIdx.x == 0) *status = bad ? kStatusBadCuSeqlens : kStatusOk;
+  }
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, j = lane % kLanes;
   const int parts = p.P / kRows;
   const int chain = static_cast<int>(blockIdx.x) / parts, part = static_cast<int>(blockIdx.x) - chain * parts;
@@ -130,17 +138,17 @@ __global__ void __launch_bounds__(kThreads) ssm_step_kernel(const SsmParams p, i
 }
 
 template <int kNs>
-cudaError_t launch(const SsmParams& p, int most, cudaStream_t stream) {
+cudaError_t launch(const SsmParams& p, int most, int* status, cudaStream_t stream) {
   const int64_t blocks = static_cast<int64_t>(p.N) * p.H * (p.P / (kNs == 128 ? 32 : 64));
   auto kernel = p.cu_seqlens != nullptr ? (p.state_fp32 ? ssm_step_kernel<kNs, true, true> : ssm_step_kernel<kNs, false, true>)
                                         : (p.state_fp32 ? ssm_step_kernel<kNs, true, false> : ssm_step_kernel<kNs, false, false>);
-  return launch_after(kernel, dim3(static_cast<unsigned>(blocks)), kThreads, 0, stream, p, most);
+  return launch_after(kernel, dim3(static_cast<unsigned>(blocks)), kThreads, 0, stream, p, most, status);
 }
 
 }  // namespace ssm_step
 
-cudaError_t launch_ssm_step(const SsmParams& p, int most, cudaStream_t stream) {
-  return p.Ns == 128 ? ssm_step::launch<128>(p, most, stream) : ssm_step::launch<64>(p, most, stream);
+cudaError_t launch_ssm_step(const SsmParams& p, int most, int* status, cudaStream_t stream) {
+  return p.Ns == 128 ? ssm_step::launch<128>(p, most, status, stream) : ssm_step::launch<64>(p, most, status, stream);
 }
 
 }  // namespace fkda

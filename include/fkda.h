@@ -220,7 +220,7 @@ typedef struct fkda_ssm_params {
   const void* initial_state; /* [N][H][P][Ns] of state_dtype, or NULL: zeros */
   void* final_state;         /* same shape and dtype, or NULL; may be initial_state itself */
   const int64_t* cu_seqlens; /* device int64 [N+1], or NULL for B sequences of T tokens */
-  void* workspace;           /* >= fkda_ssm_scratch_bytes bytes, 256-byte aligned (NULL where that is 0) */
+  void* workspace;           /* >= fkda_ssm_scratch_bytes bytes, 256-byte aligned (may be NULL where that is 0) */
   int64_t workspace_bytes;
   int64_t B;
   int64_t T;
@@ -243,7 +243,8 @@ typedef struct fkda_ssm_params {
   uint32_t flags;            /* 0 or FKDA_FLAG_STATUS_UNREAD */
 } fkda_ssm_params;
 /* Bytes of workspace that fkda_ssm_fwd needs for these sizes, on the current device (data pointers other than cu_seqlens are not looked at):
- * 0 for equal lengths of at most 16 tokens.  Its first word is the call's status, as fkda_read_status reads it. */
+ * 0 where T is at most 16, packed batches included.  Its first word is the call's status, as fkda_read_status reads it; calls that need no scratch memory
+ * write the word where a workspace of at least four bytes is given (256-byte aligned, too), and report nothing without one. */
 int fkda_ssm_scratch_bytes(const fkda_ssm_params* p, int64_t* bytes);
 int fkda_ssm_fwd(const fkda_ssm_params* p, void* cuda_stream);
 

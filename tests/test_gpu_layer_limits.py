@@ -1,10 +1,11 @@
-"""GPU: the operators round the recurrence where their numbers get hard."""
+"""GPU: the operators round the recurrence where their numbers get hard, and where a call follows one that failed."""
 import pytest
 import torch
 
 import flashkda_b200 as F
 import layer_ref as R
 from test_gpu_conv_norm import norm_bound, randn
+from test_gpu_ssm import inputs
 
 pytestmark = pytest.mark.gpu
 bf16, fp32 = torch.bfloat16, torch.float32
@@ -27,3 +28,35 @@ def test_gated_norm_where_x_times_gate_overflows(act, gate_first, D):
     if not gate_first:                                              # the square of 1e25 is beyond fp32 itself, whatever the gate
         out, want = out[:, 1:], want[:, 1:]
     assert R.off(out, want, norm_bound(want)) <= 1
+
+
+@pytest.mark.parametrize("bad,T", [([0, 400, 0, 400, 100], 400), ([0, 9, 300], 200)])
+@pytest.mark.parametrize("lens", [None, [2, 1, 4]])
+def test_status_of_a_step_behind_a_call_that_failed(bad, T, lens):
+    """A fixed workspace: a good step after a batch whose cu_seqlens were bad reads as good, through every route of few tokens."""
+    x, dt, Bm, Cm, A_log, dt_bias, D, _ = inputs(1, T, 2, 64, 1, 128)
+    cu = torch.tensor(bad, device="cuda")
+    args = (x, dt, Bm, Cm, torch.empty_like(x), A_log, dt_bias, D, None, None, cu)
+    ws = torch.empty(F.ssm_workspace_size(*args), dtype=torch.uint8, device="cuda")
+    F.ssm_fwd(*args, workspace=ws)
+    with pytest.raises(RuntimeError, match="not monotone"):
+        F.read_status(ws)
+    n = 1 if lens is None else sum(lens)
+    cu = None if lens is None else torch.tensor([0] + torch.tensor(lens).cumsum(0).tolist(), device="cuda")
+    out = torch.empty_like(x[:, :n])
+    F.ssm_fwd(x[:, :n], dt[:, :n], Bm[:, :n], Cm[:, :n], out, A_log, dt_bias, D, cu_seqlens=cu, workspace=ws)
+    assert F.read_status(ws) == 0
+    plain = torch.empty_like(out)
+    F.ssm_fwd(x[:, :n], dt[:, :n], Bm[:, :n], Cm[:, :n], plain, A_log, dt_bias, D, cu_seqlens=cu)
+    assert torch.equal(out, plain)
+
+
+@pytest.mark.parametrize("bad", [[0, 9, 4, 12], [0, 5, 13], [-1, 4, 12], [3, 2, 12]])
+def test_bad_cu_seqlens_of_few_tokens_are_reported(bad):
+    x, dt, Bm, Cm, A_log, dt_bias, D, _ = inputs(1, 12, 2, 64, 1, 128)
+    ws = torch.zeros(256, dtype=torch.uint8, device="cuda")
+    F.ssm_fwd(x, dt, Bm, Cm, torch.empty_like(x), A_log, dt_bias, D, cu_seqlens=torch.tensor(bad, device="cuda"), workspace=ws)
+    with pytest.raises(RuntimeError, match="not monotone"):
+        F.read_status(ws)
+    F.ssm_fwd(x, dt, Bm, Cm, torch.empty_like(x), A_log, dt_bias, D, cu_seqlens=torch.tensor([0, 5, 12], device="cuda"), workspace=ws)
+    assert F.read_status(ws) == 0

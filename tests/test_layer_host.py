@@ -129,3 +129,8 @@ def test_cpu_tensors_are_refused_not_computed():
         F.add_norm(z(1, 4, 64), z(1, 4, 64), z(64), z(1, 4, 64), z(1, 4, 64))
     with pytest.raises(RuntimeError, match="must be a tensor"):
         F.add_norm(None, z(1, 4, 64), z(64), z(1, 4, 64), z(1, 4, 64))
+
+
+def test_a_workspace_of_a_short_scan_has_to_be_aligned():
+    """It holds the status word, though nothing else is asked for."""
+    refused("fkda_ssm_fwd", ssm(T=4, x_batch_stride=1024, out_batch_stride=1024, workspace=G + 16, workspace_bytes=256), "256-byte aligned")
