@@ -19,7 +19,8 @@
 // token's weight as wh + wl: hi = round(x wh), whose error x wh - hi is a bf16 number itself, and lo = round((x wh - hi) + x wl): three
 // instructions for two elements, where unpacking, an fp32 product and two conversions took eight.
 // Decays: every exponent that is evaluated is a sum of terms of one sign, so that nothing cancels, but for those within 32 x 32 blocks on
-// the diagonal, which are differences of sums over less than 32 tokens.
+// the diagonal that lose less than 2^-100: there M's factor is 2^p_i 2^-p_j delta_j, off by 2^-24 of the running sums p, 1e-5 at most.  In blocks that lose
+// more each row adds up its own exponents from the diagonal backwards (a step that resets the state leaves those behind it as they are).
 // Rows past a sequence's end are zeroed in the tiles of x and B where they are summed over; those of C only reach outputs that are not stored.
 //
 // What bounds it (4 x 8192 tokens, 32 heads of P = Ns = 128: 128 CTAs of 64 blocks, 208 us on tensors that are new each time, 180 over and over; 572 MB,
@@ -54,12 +55,13 @@ constexpr uint32_t kColG = 0, kColY = 128, kColX = 256 /* hi, then lo */, kColS 
 // Per block and head, written by warps 16 and 18.
 struct Scalars {
   float p[2][kQ];          // running sum of a from the start of the token's 32-token block, itself included
-  float g[2][kQ];          // delta 2^-p; where the block's sum is beyond kMostDecay instead p - log2(delta)
+  float g[2][kQ];          // delta 2^-p; where the block's sum is beyond kMostDecay delta itself
   float f[2][kQ];          // delta 2^(sum of a behind the token to the end of its 32-token block)
   uint2 w[2][kQ / 2];      // f decayed to the end of the block of 128, two tokens a word: as bf16, and what that leaves as bf16
   float tot[2][4];         // sums over the four 32-token blocks
   float decay[2];          // 2^(sum over all)
-  float pad[6];
+  float rate[2];           // a of a delta of 1
+  float pad[4];
 };
 
 // Decay within a 32-token block up to which 2^(p_i - p_j) is taken as 2^p_i 2^-p_j: both factors, and delta with them, stay normal numbers.
@@ -152,6 +154,49 @@ __device__ __forceinline__ void keep_triangle(uint32_t (&m)[16], const uint8_t* 
   }
 }
 
+// Whether a head's M of the 32 x 32 block on the diagonal has to take its exponents one by one.
+__device__ __forceinline__ bool forgets(const Scalars& s, int h, int block) { return !(s.tot[h][block] >= kMostDecay); }
+// (powers that are multiplied: of a row's running sum and of a column's own)
+__device__ __forceinline__ void weigh_m(uint32_t (&m)[16], const uint32_t (&g)[32], float r, const float* column) {
+  const float e = ex2f(r);
+  const f2 r2 = pk(e, e);
+  const float4* f = reinterpret_cast<const float4*>(column);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float4 v = f[j];
+    m[2 * j] = round2(mul(pk(g[4 * j], g[4 * j + 1]), mul(r2, pk(v.x, v.y))));
+    m[2 * j + 1] = round2(mul(pk(g[4 * j + 2], g[4 * j + 3]), mul(r2, pk(v.z, v.w))));
+  }
+}
+// The block (w, w) where a head forgets.  Apart from make_m, which then is no longer in the instruction caches' way (5 % of a packed batch).
+template <bool kWide>
+__device__ __noinline__ void make_m_one_by_one(uint32_t at, const Scalars& s, int w, const uint8_t* masks) {
+  const int lane = threadIdx.x & 31;
+  uint32_t g[32];
+  tmem_ld32(at, g);
+  tmem_wait_ld();
+#pragma unroll 1
+  for (int h = 0; h < (kWide ? 1 : 2); ++h) {
+    uint32_t m[16];
+    if (forgets(s, h, w)) {
+      const float2* delta = reinterpret_cast<const float2*>(s.g[h] + 32 * w);
+      const float rate = s.rate[h];
+      float sum = 0.f;                                                // of a behind the column's token up to the row's
+#pragma unroll
+      for (int j = 15; j >= 0; --j) {
+        const float2 d = delta[j];
+        const float hi = __uint_as_float(g[2 * j + 1]) * (ex2f(sum) * d.y);
+        if (2 * j + 1 <= lane) sum = fmaf(rate, d.y, sum);
+        m[j] = pack_bf16(__uint_as_float(g[2 * j]) * (ex2f(sum) * d.x), hi);
+        if (2 * j <= lane) sum = fmaf(rate, d.x, sum);
+      }
+    } else {
+      weigh_m(m, g, s.p[h][32 * w + lane], s.g[h] + 32 * w);
+    }
+    keep_triangle(m, masks + lane * kMaskPitch);
+    tmem_st16(at + 16 * h, m);
+  }
+}
 // M of the 32 x 32 block (w, b) from G, over it: 16 columns a head.  (One copy for all sixteen warps that make M: see wait_on.)
 template <bool kWide>
 __device__ __noinline__ void make_m(uint32_t at, const Scalars& s, int b, int w, const uint8_t* masks) {
@@ -164,6 +209,7 @@ __device__ __noinline__ void make_m(uint32_t at, const Scalars& s, int b, int w,
     tmem_st32(at, g);
     return;
   }
+  if (b == w && (forgets(s, 0, w) || (!kWide && forgets(s, 1, w)))) return make_m_one_by_one<kWide>(at, s, w, masks);
   tmem_ld32(at, g);
   tmem_wait_ld();
 #pragma unroll 1
@@ -172,25 +218,7 @@ __device__ __noinline__ void make_m(uint32_t at, const Scalars& s, int b, int w,
     const float4 tot = *reinterpret_cast<const float4*>(s.tot[h]);
     // (with the sums over the 32-token blocks between the two)
     const float r = s.p[h][32 * w + lane] + (b < 1 && w > 1 ? tot.y : 0.f) + (b < 2 && w > 2 ? tot.z : 0.f);
-    if (b < w || (w == 0 ? tot.x : w == 1 ? tot.y : w == 2 ? tot.z : tot.w) >= kMostDecay) {
-      const float e = ex2f(r);
-      const f2 r2 = pk(e, e);
-      const float4* f = reinterpret_cast<const float4*>((b < w ? s.f[h] : s.g[h]) + 32 * b);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float4 v = f[j];
-        m[2 * j] = round2(mul(pk(g[4 * j], g[4 * j + 1]), mul(r2, pk(v.x, v.y))));
-        m[2 * j + 1] = round2(mul(pk(g[4 * j + 2], g[4 * j + 3]), mul(r2, pk(v.z, v.w))));
-      }
-    } else {
-      // (differences of exponents that have to be taken before the power)
-      const float2* lp = reinterpret_cast<const float2*>(s.g[h] + 32 * b);
-#pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const float2 v = lp[j];
-        m[j] = pack_bf16(__uint_as_float(g[2 * j]) * ex2f(r - v.x), __uint_as_float(g[2 * j + 1]) * ex2f(r - v.y));
-      }
-    }
+    weigh_m(m, g, r, (b < w ? s.f[h] : s.g[h]) + 32 * b);
     if (b == w) keep_triangle(m, masks + lane * kMaskPitch);
     tmem_st16(at + 16 * h, m);
   }
@@ -689,11 +717,12 @@ __global__ void __launch_bounds__(kThreads, 1) ssm_scan_kernel(const __grid_cons
         const float p0 = head_sum + a[0], p1 = p0 + a[1], p2 = p1 + a[2], p3 = p2 + a[3];
         reinterpret_cast<float4*>(s.p[h])[lane] = make_float4(p0, p1, p2, p3);
         reinterpret_cast<float4*>(s.g[h])[lane] = whole >= kMostDecay ? make_float4(d[0] * ex2f(-p0), d[1] * ex2f(-p1), d[2] * ex2f(-p2), d[3] * ex2f(-p3))
-                                                                      : make_float4(p0 - __log2f(d[0]), p1 - __log2f(d[1]), p2 - __log2f(d[2]), p3 - __log2f(d[3]));
+                                                                      : make_float4(d[0], d[1], d[2], d[3]);
         reinterpret_cast<float4*>(s.f[h])[lane] = f;
         if (lane == 0) {
           *reinterpret_cast<float4*>(s.tot[h]) = make_float4(t0, t1, t2, t3);
           s.decay[h] = ex2f(sum);
+          s.rate[h] = A;
         }
       }
       __syncwarp();

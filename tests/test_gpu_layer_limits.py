@@ -1,11 +1,11 @@
-"""GPU: the operators round the recurrence where their numbers get hard, and where a call follows one that failed."""
+"""GPU: the operators round the recurrence where their numbers get hard - resets, products that overflow on the way - and where a call follows one that failed."""
 import pytest
 import torch
 
 import flashkda_b200 as F
 import layer_ref as R
 from test_gpu_conv_norm import norm_bound, randn
-from test_gpu_ssm import inputs
+from test_gpu_ssm import check, exponent_slack, inputs
 
 pytestmark = pytest.mark.gpu
 bf16, fp32 = torch.bfloat16, torch.float32
@@ -60,3 +60,26 @@ def test_bad_cu_seqlens_of_few_tokens_are_reported(bad):
         F.read_status(ws)
     F.ssm_fwd(x, dt, Bm, Cm, torch.empty_like(x), A_log, dt_bias, D, cu_seqlens=torch.tensor([0, 5, 12], device="cuda"), workspace=ws)
     assert F.read_status(ws) == 0
+
+
+def with_resets(T, H, P, G, Ns, every, size, seed):
+    """Steps of `size` at every `every`th token, of some 1e-3 between: what was before is forgotten at once, what comes behind is kept.  The resets add nothing (x = 0)."""
+    x, dt, Bm, Cm, A_log, dt_bias, D, x0 = inputs(1, T, H, P, G, Ns, seed=seed, state="fp32")
+    dt_bias.zero_()
+    dt = (torch.randn(1, T, H, generator=torch.Generator().manual_seed(seed)) * 0.5 - 7.0).to(bf16).cuda()
+    at = torch.arange(T) % every == 3
+    dt[:, at] = size
+    x[:, at] = 0.0
+    return x, dt, Bm, Cm, A_log, dt_bias, D, x0
+
+
+@pytest.mark.parametrize("size", [20.0, 300.0, 1e4, 1e6, 1e12, 1e30])
+@pytest.mark.parametrize("T,every,P,Ns", [(200, 37, 64, 128), (130, 9, 128, 64), (400, 150, 64, 64)])
+def test_steps_that_reset_the_state(T, every, P, Ns, size):
+    """The decays between the tokens behind a reset do not depend on how far the reset went."""
+    args = with_resets(T, 4, P, 2, Ns, every, size, seed=T)
+    x, dt, Bm, Cm, A_log, dt_bias, D, x0 = args
+    want, mass, last, lmass = R.ssm(*args, None)
+    out, fin = torch.full_like(x, float("nan")), torch.full_like(x0, float("nan"))
+    F.ssm_fwd(x, dt, Bm, Cm, out, A_log, dt_bias, D, initial_state=x0, final_state=fin)
+    check(out, fin, want, mass, last, lmass, T, None, False, exponent_slack(A_log, dt, dt_bias, None))
