@@ -55,17 +55,18 @@ constexpr uint32_t kColG = 0, kColY = 128, kColX = 256 /* hi, then lo */, kColS 
 // Per block and head, written by warps 16 and 18.
 struct Scalars {
   float p[2][kQ];          // running sum of a from the start of the token's 32-token block, itself included
-  float g[2][kQ];          // delta 2^-p; where the block's sum is beyond kMostDecay delta itself
+  float g[2][kQ];          // delta 2^-p; where the block's sum is beyond `most` delta itself
   float f[2][kQ];          // delta 2^(sum of a behind the token to the end of its 32-token block)
   uint2 w[2][kQ / 2];      // f decayed to the end of the block of 128, two tokens a word: as bf16, and what that leaves as bf16
   float tot[2][4];         // sums over the four 32-token blocks
   float decay[2];          // 2^(sum over all)
   float rate[2];           // a of a delta of 1
-  float pad[4];
+  float most[2];           // sum of a over a 32-token block up to which decays within it are products of powers
+  float pad[2];
 };
 
-// Decay within a 32-token block up to which 2^(p_i - p_j) is taken as 2^p_i 2^-p_j: both factors, and delta with them, stay normal numbers.
-constexpr float kMostDecay = -100.f;
+// Decay within a 32-token block up to which 2^(p_i - p_j) is taken as 2^p_i 2^-p_j, and sum of its deltas: both factors, with delta, stay normal numbers.
+constexpr float kMostDecay = -100.f, kMostDelta = 134217728.f;
 // Masks of a 32 x 32 triangle for pairs of bf16: row i, 16 words, rows 80 bytes apart (16-byte reads of eight rows then meet no bank twice).
 constexpr int kMaskPitch = 80;
 
@@ -155,7 +156,7 @@ __device__ __forceinline__ void keep_triangle(uint32_t (&m)[16], const uint8_t* 
 }
 
 // Whether a head's M of the 32 x 32 block on the diagonal has to take its exponents one by one.
-__device__ __forceinline__ bool forgets(const Scalars& s, int h, int block) { return !(s.tot[h][block] >= kMostDecay); }
+__device__ __forceinline__ bool forgets(const Scalars& s, int h, int block) { return !(s.tot[h][block] >= s.most[h]); }
 // (powers that are multiplied: of a row's running sum and of a column's own)
 __device__ __forceinline__ void weigh_m(uint32_t (&m)[16], const uint32_t (&g)[32], float r, const float* column) {
   const float e = ex2f(r);
@@ -714,15 +715,17 @@ __global__ void __launch_bounds__(kThreads, 1) ssm_scan_kernel(const __grid_cons
       reinterpret_cast<uint4*>(s.w[h])[lane] = w;
       if constexpr (kFull) {
         const float whole = block == 0 ? t0 : block == 1 ? t1 : block == 2 ? t2 : t3;
+        const float most = fmaxf(kMostDecay, A * kMostDelta);
         const float p0 = head_sum + a[0], p1 = p0 + a[1], p2 = p1 + a[2], p3 = p2 + a[3];
         reinterpret_cast<float4*>(s.p[h])[lane] = make_float4(p0, p1, p2, p3);
-        reinterpret_cast<float4*>(s.g[h])[lane] = whole >= kMostDecay ? make_float4(d[0] * ex2f(-p0), d[1] * ex2f(-p1), d[2] * ex2f(-p2), d[3] * ex2f(-p3))
+        reinterpret_cast<float4*>(s.g[h])[lane] = whole >= most ? make_float4(d[0] * ex2f(-p0), d[1] * ex2f(-p1), d[2] * ex2f(-p2), d[3] * ex2f(-p3))
                                                                       : make_float4(d[0], d[1], d[2], d[3]);
         reinterpret_cast<float4*>(s.f[h])[lane] = f;
         if (lane == 0) {
           *reinterpret_cast<float4*>(s.tot[h]) = make_float4(t0, t1, t2, t3);
           s.decay[h] = ex2f(sum);
           s.rate[h] = A;
+          s.most[h] = most;
         }
       }
       __syncwarp();

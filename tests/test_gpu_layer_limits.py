@@ -83,3 +83,16 @@ def test_steps_that_reset_the_state(T, every, P, Ns, size):
     out, fin = torch.full_like(x, float("nan")), torch.full_like(x0, float("nan"))
     F.ssm_fwd(x, dt, Bm, Cm, out, A_log, dt_bias, D, initial_state=x0, final_state=fin)
     check(out, fin, want, mass, last, lmass, T, None, False, exponent_slack(A_log, dt, dt_bias, None))
+
+
+@pytest.mark.parametrize("size", [1e6, 1e9, 1e12, 1e18, 1e25])
+def test_large_steps_with_rates_as_small(size):
+    """Steps beyond 2^27 whose decays are those of ordinary ones, on inputs as small as the steps are large."""
+    x, dt, Bm, Cm, A_log, dt_bias, D, x0 = inputs(1, 150, 4, 64, 1, 128, seed=8, state="fp32")
+    dt[:] = (size * torch.rand(1, 150, 4, generator=torch.Generator().manual_seed(1))).to(bf16).cuda()
+    A_log = torch.log(torch.tensor([0.01, 1.0, 2.0, 4.5], dtype=torch.float64) / size).float().cuda()      # (whole 32-token blocks lose 2^-0.2 to 2^-104)
+    x = (x.float() / size).to(bf16)
+    want, mass, last, lmass = R.ssm(x, dt, Bm, Cm, A_log, dt_bias, D, x0, None)
+    out, fin = torch.full_like(x, float("nan")), torch.full_like(x0, float("nan"))
+    F.ssm_fwd(x, dt, Bm, Cm, out, A_log, dt_bias, D, initial_state=x0, final_state=fin)
+    check(out, fin, want, mass, last, lmass, 150, None, False, exponent_slack(A_log, dt, dt_bias, None))
