@@ -15,9 +15,12 @@
 //     16, 18 delta and the decays, a head each       17     products       19     tensor copies (beside the rows of M with the most to do)
 //
 // Roundings: all products accumulate in fp32.  M and the state's copy are bf16 operands, as out is bf16.  The state is what a
-// caller keeps, so X' goes into its product as hi + lo, two bf16 parts that hold 16 bits.  They come straight from x, which is bf16, and the
-// token's weight as wh + wl: hi = round(x wh), whose error x wh - hi is a bf16 number itself, and lo = round((x wh - hi) + x wl): three
-// instructions for two elements, where unpacking, an fp32 product and two conversions took eight.
+// caller keeps, so X' goes into its product in parts: three bf16 numbers, which hold fp32's 24 bits, where the caller gets an fp32 state; two (16 bits) where
+// it is rounded to bf16 or not asked for.  The parts come straight from x, which is bf16, and the token's weight as w0 + w1 (+ w2), in operations on bf16 pairs:
+//     h = round(x w0),  e = x w0 - h, a bf16 number itself;   two parts: h and round(e + x w1)
+//     three parts: m = round(e + round(x w1));  m - e is a bf16 number too (e is a multiple of the last bit of round(x w1));  l = round(round(x w1 - (m - e)) + x w2)
+// Three instructions for two elements, and seven; taken apart in fp32 it was eight and twelve.  Against 64 bits the final state of 4 x 8192 x 32 x 128 is off by 2.4e-7
+// of its norm with three parts, and would be by 4.7e-6 with two (242 us for 207).
 // Decays: every exponent that is evaluated is a sum of terms of one sign, so that nothing cancels, but for those within 32 x 32 blocks on
 // the diagonal that lose less than 2^-100: there M's factor is 2^p_i 2^-p_j delta_j, off by 2^-24 of the running sums p, 1e-5 at most.  In blocks that lose
 // more each row adds up its own exponents from the diagonal backwards (a step that resets the state leaves those behind it as they are).
@@ -50,14 +53,22 @@ constexpr int kThreads = 20 * 32;          // (registers are given to four warps
 constexpr int kTileX = kQ * 128 * 2;
 constexpr int kXs = 3;                           // tiles of x: one being read, one with its output on the way out, one on the way in
 constexpr int kScals = 4;                        // blocks whose decays are at hand: they are worked out ahead
-constexpr uint32_t kColG = 0, kColY = 128, kColX = 256 /* hi, then lo */, kColS = 384;     // tensor memory; M lies over G
+constexpr uint32_t kColG = 0, kColY = 128, kColX = 256, kColS = 384;     // tensor memory; M lies over G
+// X'^T over 32 tokens (a quarter of a block) takes 16 columns a part, in the order of the products: the last part first.  The full pass has room for eight such pieces: all
+// of two parts, two thirds of three.
+template <int kParts, bool kFull>
+__device__ __forceinline__ uint32_t piece_column(int quarter, int part) {
+  const int piece = quarter * kParts + kParts - 1 - part;
+  return 16 * piece + (kFull ? kColX - (piece >= 8 ? 128 : 0) : 0);
+}
 
 // Per block and head, written by warps 16 and 18.
 struct Scalars {
   float p[2][kQ];          // running sum of a from the start of the token's 32-token block, itself included
   float g[2][kQ];          // delta 2^-p; where the block's sum is beyond `most` delta itself
   float f[2][kQ];          // delta 2^(sum of a behind the token to the end of its 32-token block)
-  uint2 w[2][kQ / 2];      // f decayed to the end of the block of 128, two tokens a word: as bf16, and what that leaves as bf16
+  uint2 w[2][kQ / 2];      // f decayed to the end of the block of 128, two tokens a word: as bf16, and what that leaves as bf16,
+  uint32_t rest[2][kQ / 2];        // and (three parts) what that leaves
   float tot[2][4];         // sums over the four 32-token blocks
   float decay[2];          // 2^(sum over all)
   float rate[2];           // a of a delta of 1
@@ -81,10 +92,10 @@ static_assert(Smem<128>::kBytes <= 227 * 1024, "shared memory of a CTA");
 
 enum {
   B_FULL_B = 0, B_FULL_C, B_Z /* C S^T done, C free */, B_FULL_X /*[kXs]*/, B_EMPTY_X = 6 /*[kXs]*/, B_OUT = 9 /*[kXs]*/, B_XT = 12 /*[2]*/, B_SCAL = 14 /*[kScals]*/,
-  B_SCAL_FREE = 18 /*[kScals]*/, B_G = 22, B_Y, B_M, B_Y_FREE, B_S_FULL /* X'^T B done, B free */, B_S_READY, B_DRAIN, B_MEET, B_COUNT,
+  B_SCAL_FREE = 18 /*[kScals]*/, B_G = 22, B_Y, B_M, B_Y_FREE, B_S_FULL /* X'^T B done, B free */, B_S_READY, B_DRAIN, B_MEET, B_XT_FREE /*[2]*/, B_COUNT = B_XT_FREE + 2,
   B_EMPTY_B = B_G, B_XT2 = B_OUT      // of the first pass, [2] each: buffer c & 1 of B and X'^T free; X'^T of the second buffer
 };
-static_assert(B_COUNT * 8 <= 256, "barrier area");
+static_assert(B_COUNT <= 32, "a lane each to make them, 256 bytes");
 
 // Arrivals that complete a phase of barrier `i`.
 template <bool kFull, bool kWide>
@@ -130,10 +141,26 @@ __device__ __forceinline__ uint32_t mul_bf2(uint32_t a, uint32_t b) {
   asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
+__device__ __forceinline__ uint32_t add_bf2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t sub_bf2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
 __device__ __forceinline__ uint32_t fma_bf2(uint32_t a, uint32_t b, uint32_t c) {
   uint32_t r;
   asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
   return r;
+}
+// 16 TMEM lanes x 16 columns (the shape of tmem_st_16x128b_x8, half of it).
+__device__ __forceinline__ void tmem_st_16x128b_x4(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.16x128b.x4.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]),
+               "r"(r[6]), "r"(r[7])
+               : "memory");
 }
 using elem::f2;
 using elem::fma2;
@@ -258,8 +285,8 @@ __device__ __noinline__ void leave_state(uint32_t at, uint32_t rows, void* dst) 
   fence_proxy_async_smem();                       // (tensor copies write there next)
 }
 
-// kWide: one head of P = 128, else two of P = 64.  kFull: the outputs too, else only what a run adds to a zero state.
-template <int kNs, bool kWide, bool kFull>
+// kWide: one head of P = 128, else two of P = 64.  kFull: the outputs too, else only what a run adds to a zero state.  kParts: of X', two or three.
+template <int kNs, bool kWide, bool kFull, int kParts>
 __global__ void __launch_bounds__(kThreads, 1) ssm_scan_kernel(const __grid_constant__ SsmMaps maps, const SsmScanParams p) {
   using L = Smem<kNs>;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -414,38 +441,48 @@ __global__ void __launch_bounds__(kThreads, 1) ssm_scan_kernel(const __grid_cons
     auto state_at = [&](int r) { return ((static_cast<int64_t>(it.n) * p.H + it.head0 + h) * (kWide ? 128 : 64) + (kWide ? r : r & 63)) * kNs + g * kOwn; };
     float4* slot = it.slot >= 0 ? p.slots + static_cast<int64_t>(it.slot) * (128 * kNs / 4) + (g * kOwn / 4) * 128 + row : nullptr;       // (four columns of a row, 128 further on the next four)
     const int t = tid - 8 * 32;
-    // X'^T: this warp's 16 rows of 32, 64 tokens at a time.  A transposed 8 x 8 tile of x has two tokens of a channel in a register, as
-    // tensor memory wants them (register 2j | 2j + 1: lane t/4 | t/4 + 8, column 4j + t%4).
-    auto weigh = [&](uint32_t x, const Scalars& s, uint32_t column, int done) {
-      const uint32_t src = x + ((warp & 3) >> 1) * (kTileX / 2) + (8 * (lane >> 4) + (lane & 7)) * 128 + (((4 * (warp & 1) + 2 * g + ((lane >> 3) & 1)) ^ (lane & 7)) << 4);
-      const uint32_t xt = tmem + (static_cast<uint32_t>(32 * (warp & 3) + 16 * g) << 16) + column;
-#pragma unroll 1
-      for (int th = 0; th < 2; ++th) {
-        uint32_t hi[16], lo[16];
+    // X'^T over 64 tokens, this warp's 16 rows of 32, 32 tokens at a time.  A transposed 8 x 8 tile of x has two tokens of a channel in a register,
+    // as tensor memory wants them (register 2j | 2j + 1: lane t/4 | t/4 + 8, column 4j + t%4).
+    uint32_t part[2][kParts][8];
+    auto weigh = [&](uint32_t x, const Scalars& s, int half) {
+      const uint32_t src = x + ((warp & 3) >> 1) * (kTileX / 2) + (64 * half + 8 * (lane >> 4) + (lane & 7)) * 128 + (((4 * (warp & 1) + 2 * g + ((lane >> 3) & 1)) ^ (lane & 7)) << 4);
+      const uint2* w = s.w[kWide ? 0 : h] + 32 * half + (lane & 3);
+      const uint32_t* rest = s.rest[kWide ? 0 : h] + 32 * half + (lane & 3);
+      __syncwarp();
 #pragma unroll
-        for (int j = 0; j < 8; j += 2) ldsm_x4_trans(src + (64 * th + 8 * j) * 128, hi[2 * j], hi[2 * j + 1], hi[2 * j + 2], hi[2 * j + 3]);
-        const uint2* w = s.w[kWide ? 0 : h] + 32 * th + (lane & 3);
+      for (int q = 0; q < 2; ++q) {
+        uint32_t (&first)[8] = part[q][0];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const uint2 wj = w[4 * j];
+        for (int j = 0; j < 4; j += 2) ldsm_x4_trans(src + (32 * q + 8 * j) * 128, first[2 * j], first[2 * j + 1], first[2 * j + 2], first[2 * j + 3]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint2 wj = w[16 * q + 4 * j];
+          const uint32_t minus = wj.x ^ 0x80008000u, rj = kParts == 3 ? rest[16 * q + 4 * j] : 0u;
 #pragma unroll
           for (int i = 2 * j; i < 2 * j + 2; ++i) {
-            const uint32_t xi = hi[i];
-            hi[i] = mul_bf2(xi, wj.x);
-            lo[i] = fma_bf2(xi, wj.y, fma_bf2(xi, wj.x, hi[i] ^ 0x80008000u));
+            const uint32_t xi = first[i];
+            first[i] = mul_bf2(xi, minus);                              // (the first part is minus what it stands for; the products have the sign)
+            const uint32_t err = fma_bf2(xi, wj.x, first[i]);
+            if constexpr (kParts == 2) {
+              part[q][1][i] = fma_bf2(xi, wj.y, err);
+            } else {
+              part[q][1][i] = add_bf2(err, mul_bf2(xi, wj.y));
+              part[q][2][i] = fma_bf2(xi, rj, fma_bf2(xi, wj.y, sub_bf2(err, part[q][1][i])));
+            }
           }
         }
-        tmem_st_16x128b_x8(xt + 32 * th, hi);
-        tmem_st_16x128b_x8(xt + 64 + 32 * th, lo);
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(done + th));
       }
+    };
+    auto put = [&](int quarter, int q, int k) { tmem_st_16x128b_x4(tmem + (static_cast<uint32_t>(32 * (warp & 3) + 16 * g) << 16) + piece_column<kParts, kFull>(quarter, k), part[q][k]); };
+    auto stored = [&](int done) {
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(done));
     };
     if constexpr (!kFull) {
       // First pass: from the run's last block to its first, with weights that decay to the run's end, so that nothing is ever rescaled.
-      // Two buffers of X'^T (the second one where G would be) and of B.
+      // Two buffers of X'^T (from column 0 on: there is no G, M or output) and of B.
       for (int c = 0; c < blocks; ++c) {
         if (!(ok = warp_wait(bar(B_SCAL + c % kScals), (c / kScals) & 1, abort_flag))) break;
         if (!(ok = warp_wait(bar(B_FULL_X + c % kXs), (c / kXs) & 1, abort_flag))) break;
@@ -453,7 +490,15 @@ __global__ void __launch_bounds__(kThreads, 1) ssm_scan_kernel(const __grid_cons
           if (!(ok = warp_wait(bar(B_EMPTY_B + (c & 1)), ((c >> 1) - 1) & 1, abort_flag))) break;
           tc_fence_after();
         }
-        weigh(sbase + L::kX + (c % kXs) * kTileX, scal[c % kScals], c & 1 ? kColG : kColX, c & 1 ? B_XT2 : B_XT);
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {
+          weigh(sbase + L::kX + (c % kXs) * kTileX, scal[c % kScals], half);
+#pragma unroll
+          for (int q = 0; q < 2; ++q)
+#pragma unroll
+            for (int k = 0; k < kParts; ++k) put(4 * (c & 1) + 2 * half + q, q, k);
+          stored((c & 1 ? B_XT2 : B_XT) + half);
+        }
         if (lane == 0) {
           mbar_arrive(bar(B_SCAL_FREE + c % kScals));
           mbar_arrive(bar(B_EMPTY_X + c % kXs));
@@ -556,17 +601,43 @@ __global__ void __launch_bounds__(kThreads, 1) ssm_scan_kernel(const __grid_cons
           if (lane == 0) mbar_arrive(bar(B_MEET));
           if (!(ok = warp_wait(bar(B_MEET), 0, abort_flag))) break;
         }
-        weigh(x, s, kColX, B_XT);
-        if (!(ok = warp_wait(bar(B_G), c & 1, abort_flag))) break;
-        tc_fence_after();
-        make_m<kWide>(tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16) + kColG, s, 2 + g, warp & 3, smem + L::kMask);
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(bar(B_SCAL_FREE + c % kScals));
-          mbar_arrive(bar(B_M));
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {
+          weigh(x, s, half);
+          if (kParts == 3 && half == 1) {
+            // the first eight pieces are there; the last four follow the products of the first quarter, and of the second
+            put(2, 0, 2);
+            put(2, 0, 1);
+            stored(B_XT + 1);
+            if (!(ok = warp_wait(bar(B_XT_FREE), c & 1, abort_flag))) break;
+            tc_fence_after();
+            put(2, 0, 0);
+            put(3, 1, 2);
+            put(3, 1, 1);
+            stored(B_XT);
+            if (!(ok = warp_wait(bar(B_XT_FREE + 1), c & 1, abort_flag))) break;
+            tc_fence_after();
+            put(3, 1, 0);
+            stored(B_XT + 1);
+          } else {
+#pragma unroll
+            for (int q = 0; q < 2; ++q)
+#pragma unroll
+              for (int k = 0; k < kParts; ++k) put(2 * half + q, q, k);
+            stored(B_XT + half);
+          }
+          if (half == 1) {
+            if (!(ok = warp_wait(bar(B_G), c & 1, abort_flag))) break;
+            tc_fence_after();
+            make_m<kWide>(tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16) + kColG, s, 2 + g, warp & 3, smem + L::kMask);
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(B_M));
+          }
         }
+        if (!ok) break;
+        if (lane == 0) mbar_arrive(bar(B_SCAL_FREE + c % kScals));
       }
       if (ok && blocks > 0 && (ok = warp_wait(bar(B_S_FULL), (blocks - 1) & 1, abort_flag)) && there && it.last && p.final_state != nullptr) {
         tc_fence_after();
@@ -578,14 +649,12 @@ __global__ void __launch_bounds__(kThreads, 1) ssm_scan_kernel(const __grid_cons
   } else if (warp == 17) {
     // ---- products ----------------------------------------------------------------------------------------------------------------
     constexpr uint32_t idesc_g = umma_idesc_bf16(128, 128, 0, 0), idesc_s = umma_idesc_bf16(128, kNs, 0, 1), idesc_y = umma_idesc_bf16(128, kWide ? 128 : 64, 0, 1);
-    // S += X'^T B over 64 tokens: hi, then lo
-    auto add_state = [&](uint32_t b, uint32_t xt, int th, bool onto) {
-      const uint64_t db = desc_sw128(b + th * 8192, 16384);
+    constexpr uint32_t kMinusA = 1u << 13;                            // (of an instruction descriptor: A with the other sign)
+    // S += X'^T B over 32 tokens, the smallest parts first (sums are rounded towards zero)
+    auto add_part = [&](uint32_t b, int quarter, int slot, int part, bool onto) {
+      const uint64_t db = desc_sw128(b + quarter * 4096, 16384);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        umma_ts(tmem + kColS, tmem + xt + 32 * th + 8 * k, db + k * 128, idesc_s, onto || k > 0);
-        umma_ts(tmem + kColS, tmem + xt + 64 + 32 * th + 8 * k, db + k * 128, idesc_s, 1);
-      }
+      for (int k = 0; k < 2; ++k) umma_ts(tmem + kColS, tmem + piece_column<kParts, kFull>(slot, part) + 8 * k, db + k * 128, idesc_s | (part == 0 ? kMinusA : 0u), onto || k > 0);
     };
     if constexpr (!kFull) {
       for (int c = 0; c < blocks; ++c) {
@@ -594,7 +663,10 @@ __global__ void __launch_bounds__(kThreads, 1) ssm_scan_kernel(const __grid_cons
           if (!(ok = warp_wait(bar((c & 1 ? B_XT2 : B_XT) + th), (c >> 1) & 1, abort_flag))) break;
           tc_fence_after();
           if (elect_one()) {
-            add_state(sbase + L::kB + (c & 1) * L::kTile, c & 1 ? kColG : kColX, th, c + th > 0);
+#pragma unroll
+            for (int q = 2 * th; q < 2 * th + 2; ++q)
+#pragma unroll
+              for (int k = kParts - 1; k >= 0; --k) add_part(sbase + L::kB + (c & 1) * L::kTile, q, 4 * (c & 1) + q, k, c + q > 0 || k + 1 < kParts);
             if (th == 1) {
               if (c + 2 < blocks) umma_commit(bar(B_EMPTY_B + (c & 1)));
               else if (c + 1 == blocks) umma_commit(bar(B_S_FULL));
@@ -628,14 +700,36 @@ __global__ void __launch_bounds__(kThreads, 1) ssm_scan_kernel(const __grid_cons
         umma_commit(bar(B_Z));
       }
       __syncwarp();
-      for (int th = 0; th < 2; ++th) {
-        if (!(ok = warp_wait(bar(B_XT + th), c & 1, abort_flag))) break;
-        tc_fence_after();
-        if (elect_one()) {
-          add_state(b, kColX, th, true);
-          if (th == 1) umma_commit(bar(B_S_FULL));
+      if constexpr (kParts == 3) {
+        // pieces 0 to 5, 6 and 7, 8 to 10, 11: as they come
+#pragma unroll
+        for (int step = 0; step < 4; ++step) {
+          if (!(ok = warp_wait(bar(B_XT + (step & 1)), step >> 1, abort_flag))) break;
+          tc_fence_after();
+          if (elect_one()) {
+            if (step == 1) umma_commit(bar(B_XT_FREE + 1));           // (the first two quarters)
+#pragma unroll
+            for (int piece = step == 0 ? 0 : step == 1 ? 6 : step == 2 ? 8 : 11; piece < (step == 0 ? 6 : step == 1 ? 8 : step == 2 ? 11 : 12); ++piece) {
+              add_part(b, piece / 3, piece / 3, 2 - piece % 3, true);
+              if (piece == 2) umma_commit(bar(B_XT_FREE));
+            }
+            if (step == 3) umma_commit(bar(B_S_FULL));
+          }
+          __syncwarp();
         }
-        __syncwarp();
+      } else {
+        for (int th = 0; th < 2; ++th) {
+          if (!(ok = warp_wait(bar(B_XT + th), c & 1, abort_flag))) break;
+          tc_fence_after();
+          if (elect_one()) {
+#pragma unroll
+            for (int q = 2 * th; q < 2 * th + 2; ++q)
+#pragma unroll
+              for (int k = kParts - 1; k >= 0; --k) add_part(b, q, q, k, true);
+            if (th == 1) umma_commit(bar(B_S_FULL));
+          }
+          __syncwarp();
+        }
       }
       if (!ok) break;
       if (!(ok = warp_wait(bar(B_FULL_X + c % kXs), (c / kXs) & 1, abort_flag))) break;
@@ -710,9 +804,11 @@ __global__ void __launch_bounds__(kThreads, 1) ssm_scan_kernel(const __grid_cons
       const float4 f = make_float4(d[0] * ex2f(s0), d[1] * ex2f(s1), d[2] * ex2f(s2), d[3] * ex2f(rest));
       const float w0 = f.x * to_end, w1 = f.y * to_end, w2 = f.z * to_end, w3 = f.w * to_end;
       const uint32_t h01 = pack_bf16(w0, w1), h23 = pack_bf16(w2, w3);
-      const uint4 w = make_uint4(h01, pack_bf16(w0 - bf_lo(h01), w1 - bf_hi(h01)), h23, pack_bf16(w2 - bf_lo(h23), w3 - bf_hi(h23)));
+      const float l0 = w0 - bf_lo(h01), l1 = w1 - bf_hi(h01), l2 = w2 - bf_lo(h23), l3 = w3 - bf_hi(h23);
+      const uint32_t l01 = pack_bf16(l0, l1), l23 = pack_bf16(l2, l3);
       if (c >= kScals && !(ok = warp_wait(bar(B_SCAL_FREE + c % kScals), (c / kScals - 1) & 1, abort_flag))) break;
-      reinterpret_cast<uint4*>(s.w[h])[lane] = w;
+      reinterpret_cast<uint4*>(s.w[h])[lane] = make_uint4(h01, l01, h23, l23);
+      if constexpr (kParts == 3) reinterpret_cast<uint2*>(s.rest[h])[lane] = make_uint2(pack_bf16(l0 - bf_lo(l01), l1 - bf_hi(l01)), pack_bf16(l2 - bf_lo(l23), l3 - bf_hi(l23)));
       if constexpr (kFull) {
         const float whole = block == 0 ? t0 : block == 1 ? t1 : block == 2 ? t2 : t3;
         const float most = fmaxf(kMostDecay, A * kMostDelta);
@@ -1038,20 +1134,20 @@ bool make_tile_map(CUtensorMap* map, const void* base, int64_t columns, int64_t 
             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int kNs, bool kWide, bool kFull>
+template <int kNs, bool kWide, bool kFull, int kParts>
 cudaError_t launch_walk(const SsmMaps& maps, const SsmScanParams& p, int64_t items, cudaStream_t stream) {
   if (items == 0) return cudaSuccess;
   static SmemOptIn opt_in;
-  auto kernel = ssm_scan_kernel<kNs, kWide, kFull>;
+  auto kernel = ssm_scan_kernel<kNs, kWide, kFull, kParts>;
   const cudaError_t e = opt_in.ensure(kernel, Smem<kNs>::kBytes);
   if (e != cudaSuccess) return e;
   const int64_t ctas = p.queue != nullptr && items > device_sm_count() ? device_sm_count() : items;
   return launch_after(kernel, dim3(static_cast<unsigned>(ctas)), kThreads, Smem<kNs>::kBytes, stream, maps, p);
 }
-template <bool kFull>
+template <bool kFull, int kParts>
 cudaError_t launch_pass(const SsmMaps& maps, const SsmScanParams& p, int Ns, int64_t items, cudaStream_t stream) {
-  if (Ns == 128) return p.P == 128 ? launch_walk<128, true, kFull>(maps, p, items, stream) : launch_walk<128, false, kFull>(maps, p, items, stream);
-  return p.P == 128 ? launch_walk<64, true, kFull>(maps, p, items, stream) : launch_walk<64, false, kFull>(maps, p, items, stream);
+  if (Ns == 128) return p.P == 128 ? launch_walk<128, true, kFull, kParts>(maps, p, items, stream) : launch_walk<128, false, kFull, kParts>(maps, p, items, stream);
+  return p.P == 128 ? launch_walk<64, true, kFull, kParts>(maps, p, items, stream) : launch_walk<64, false, kFull, kParts>(maps, p, items, stream);
 }
 
 }  // namespace ssm_scan
@@ -1139,6 +1235,7 @@ cudaError_t launch_ssm_scan(const SsmParams& q, const SsmLayout& L, const SsmAid
   p.state_fp32 = q.state_fp32;
   p.wait_limit_us = aid.wait_limit_us;
   p.stop_loads_after = aid.stop_loads_after > 0 ? aid.stop_loads_after : 0x7fffffff;
+  const bool exact = q.final_state != nullptr && q.state_fp32;        // (a state that is rounded to bf16 has no use for more than 16 bits of what is added to it)
   cudaError_t e = cudaSuccess;
   if (packed) {
     e = launch_after(ssm_scan::ssm_plan_kernel, dim3(1), ssm_scan::kPlanThreads, 0, stream, q.cu_seqlens, q.N, q.T, L.pairs, device_sm_count(), L.least, p.plan, p.status);
@@ -1150,7 +1247,7 @@ cudaError_t launch_ssm_scan(const SsmParams& q, const SsmLayout& L, const SsmAid
   if (e != cudaSuccess) return e;
   if (L.first_items > 0) {
     if (packed) p.queue = p.plan->next;
-    e = ssm_scan::launch_pass<false>(maps, p, q.Ns, L.first_items, stream);
+    e = exact ? ssm_scan::launch_pass<false, 3>(maps, p, q.Ns, L.first_items, stream) : ssm_scan::launch_pass<false, 2>(maps, p, q.Ns, L.first_items, stream);
     if (e != cudaSuccess) return e;
     const int64_t each = L.pairs * (128 * q.Ns / 1024), most = (8 * device_sm_count() + each - 1) / each;
     e = launch_after(ssm_scan::ssm_chain_kernel, dim3(static_cast<unsigned>(each * (L.chained < most ? L.chained : most))), 256, 0, stream, p, q.Ns, L.pairs);
@@ -1158,7 +1255,7 @@ cudaError_t launch_ssm_scan(const SsmParams& q, const SsmLayout& L, const SsmAid
   }
   if (packed) p.queue = p.plan->next + 1;
   p.late = !packed && L.first_items > 0;
-  return ssm_scan::launch_pass<true>(maps, p, q.Ns, L.items, stream);
+  return exact ? ssm_scan::launch_pass<true, 3>(maps, p, q.Ns, L.items, stream) : ssm_scan::launch_pass<true, 2>(maps, p, q.Ns, L.items, stream);
 }
 
 }  // namespace fkda

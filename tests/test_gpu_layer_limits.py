@@ -1,4 +1,4 @@
-"""GPU: the operators round the recurrence where their numbers get hard - resets, products that overflow on the way - and where a call follows one that failed."""
+"""GPU: the operators round the recurrence where their numbers get hard - resets, products that overflow on the way, states as exact as their type - and where a call follows one that failed."""
 import pytest
 import torch
 
@@ -96,3 +96,49 @@ def test_large_steps_with_rates_as_small(size):
     out, fin = torch.full_like(x, float("nan")), torch.full_like(x0, float("nan"))
     F.ssm_fwd(x, dt, Bm, Cm, out, A_log, dt_bias, D, initial_state=x0, final_state=fin)
     check(out, fin, want, mass, last, lmass, 150, None, False, exponent_slack(A_log, dt, dt_bias, None))
+
+
+@pytest.mark.parametrize("T,B,H,P,Ns,lens", [
+    (40, 1, 4, 64, 128, None), (128, 2, 3, 64, 64, None), (300, 1, 4, 128, 128, None), (200, 2, 2, 128, 64, None), (1500, 1, 2, 64, 128, None), (3000, 1, 2, 128, 64, None), (1, 1, 5, 64, 128, [17, 130, 260, 5]),
+    (1, 1, 2, 64, 64, [3000])])
+def test_fp32_states_are_as_exact_as_fp32(T, B, H, P, Ns, lens):
+    """The last tokens, 61 apart, are there alone (x = 0 elsewhere) with a decay that is all but 1: few terms w x B, each of which has to be there with all its bits.
+
+    In units of 2^-24: delta of arguments up to 10 in size, 32 (the sum with the bias 4, its product with log2 e and that constant 10, the exponential 4, the division 4, sums and
+    products of the logarithm 10); w = delta times two powers of all but 0, 10; its product with x taken in three parts of eight bits 4; the products of
+    these with B are exact, and their three sums, each rounded towards zero, 6, and that again for every term that is added behind it; decays of up to three blocks or a run, a power and a product each, 15."""
+    n = T if lens is None else sum(lens)
+    x, dt, Bm, Cm, A_log, dt_bias, D, _ = inputs(B, n, H, P, 1, Ns, seed=T + n)
+    A_log.fill_(-14.0)
+    keep = torch.zeros(n, dtype=torch.bool)
+    cu = None if lens is None else torch.tensor([0] + torch.tensor(lens).cumsum(0).tolist(), device="cuda")
+    ends = [n] if lens is None else cu.tolist()[1:]
+    first = [0] if lens is None else cu.tolist()[:-1]
+    terms = 0
+    for a, e in zip(first, ends):
+        at = [t for t in range(e - 1, a - 1, -61)][:4]
+        keep[at] = True
+        terms = max(terms, len(at))
+    x[:, ~keep] = 0.0
+    N = B if lens is None else len(lens)
+    want, mass, last, lmass = R.ssm(x, dt, Bm, Cm, A_log, dt_bias, D, None, None if cu is None else cu.cpu())
+    out, fin = torch.empty_like(x), torch.full((N, H, P, Ns), float("nan"), device="cuda")
+    F.ssm_fwd(x, dt, Bm, Cm, out, A_log, dt_bias, D, final_state=fin, cu_seqlens=cu)
+    steps = 32 + 10 + 4 + 6 * terms + 15
+    assert R.off(fin, last, steps * R.FP32 * lmass + 1e-30) <= 1
+
+
+@pytest.mark.parametrize("T", [300, 3000])
+@pytest.mark.parametrize("P,Ns", [(64, 128), (128, 64)])
+def test_out_does_not_depend_on_the_state_that_is_asked_for(T, P, Ns):
+    """An fp32 state is kept with more bits than one in bf16 or none: `out` is the same within the roundings of its operands."""
+    x, dt, Bm, Cm, A_log, dt_bias, D, _ = inputs(1, T, 4, P, 2, Ns, seed=T)
+    outs, fins = [], []
+    for state in (fp32, bf16, None):
+        outs.append(torch.full_like(x, float("nan")))
+        fins.append(None if state is None else torch.empty(1, 4, P, Ns, dtype=state, device="cuda"))
+        F.ssm_fwd(x, dt, Bm, Cm, outs[-1], A_log, dt_bias, D, final_state=fins[-1])
+    assert torch.equal(outs[1], outs[2])
+    # what differs is 2^-16 of what goes into the states: a few operands and results are rounded the other way
+    assert ((outs[0].double() - outs[1].double()).norm() / outs[0].double().norm()).item() <= R.BF16
+    assert ((fins[0].double() - fins[1].double()).norm() / fins[0].double().norm()).item() <= R.BF16
