@@ -130,7 +130,7 @@ def _given(**named):
     return {name: t for name, t in named.items() if t is not None}
 
 
-def _launch(function, params, device, message_of=None):
+def _launch(function, params, device):
     with torch.cuda.device(device):
         stream = ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
         _check(getattr(_lib(), function)(ctypes.byref(params), stream))

@@ -101,9 +101,6 @@ __device__ __forceinline__ float rcpf(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// 1 / (1 + e^-x) to fp32 accuracy (the tanh approximation has an absolute error that small values do not bear)
-__device__ __forceinline__ float sigmoid_exact(float x) { return rcpf(1.f + ex2f(-kLog2e * x)); }
-
 // max(x, 0) + log(1 + e^-|x|) to fp32 accuracy.  log(1 + u) = 2 atanh(z) with z = u / (2 + u) <= 1/3, by the series of atanh to z^13: what is
 // left out is below 2^-26 of the sum.
 __device__ __forceinline__ float softplus(float x) {

@@ -166,7 +166,6 @@ using elem::f2;
 using elem::fma2;
 using elem::mul;
 using elem::pk;
-using elem::upk;
 __device__ __forceinline__ f2 pk(uint32_t a, uint32_t b) { return elem::pk(__uint_as_float(a), __uint_as_float(b)); }
 __device__ __forceinline__ uint32_t round2(f2 x) { return elem::round_bf(x); }
 
