@@ -142,3 +142,15 @@ def test_out_does_not_depend_on_the_state_that_is_asked_for(T, P, Ns):
     # what differs is 2^-16 of what goes into the states: a few operands and results are rounded the other way
     assert ((outs[0].double() - outs[1].double()).norm() / outs[0].double().norm()).item() <= R.BF16
     assert ((fins[0].double() - fins[1].double()).norm() / fins[0].double().norm()).item() <= R.BF16
+
+
+@pytest.mark.parametrize("B,T,H,P,G,Ns,state", [(2, 500, 4, 64, 1, 128, "fp32"), (1, 700, 2, 128, 2, 64, "bf16"), (1, 2000, 1, 64, 1, 64, "fp32")])
+def test_out_as_a_whole(B, T, H, P, G, Ns, state):
+    """Three roundings to bf16 - M, the state's copy, out - each off by 2^-7 / sqrt(12) of a value between 1 and 2 in the mean square; on random inputs, where neither they nor the terms
+    of a sum go together, at most sqrt(3) of that, 2^-8, over all of `out`."""
+    args = inputs(B, T, H, P, G, Ns, seed=T + 1, state=state)
+    x, dt, Bm, Cm, A_log, dt_bias, D, x0 = args
+    want = R.ssm(*args, None)[0]
+    out = torch.full_like(x, float("nan"))
+    F.ssm_fwd(x, dt, Bm, Cm, out, A_log, dt_bias, D, initial_state=x0, final_state=torch.empty_like(x0))
+    assert ((out.double().cpu() - want).norm() / want.norm()).item() <= 2.0 ** -8
