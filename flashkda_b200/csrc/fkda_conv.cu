@@ -6,10 +6,10 @@
 // Bound by memory: a read and a write an element, against some 30 instructions for four (two of them on the special function unit an
 // element).  What is worked on fills 96 registers, so that an SM holds 640 threads, and one group of four rows each on its way in
 // registers was 20 KB an SM, far from enough: 4 x 8192 x 4352 took 121 us.  Rows come by asynchronous copies through shared memory instead,
-// each thread its own, four groups ahead, without a barrier: 92 us on the same tensors over and over, 6.2 TB/s read and written, and 101 on other ones
-// each time.  (Over and over: three groups ahead 94, six 92; fewer registers - 72, seven blocks an SM - cost spills, 100; groups of two rows 106;
+// each thread its own, four groups ahead, without a barrier: 92 us on the same tensors over and over, 6.2 TB/s read and written, and 105 on other ones
+// each time, 5.4 TB/s.  (Over and over: three groups ahead 94, six 92; fewer registers - 72, seven blocks an SM - cost spills, 100; groups of two rows 106;
 // prefetches into L2 in place of the copies 104.)
-// Packed sequences of 1 to 300 tokens (30 thousand x 2048 with states) take 50 us, 5.1 TB/s: a sequence's start asks memory for its borders, then for
+// Packed sequences of 1 to 300 tokens (30 thousand x 2048 with states) take 52 us, 4.9 TB/s: a sequence's start asks memory for its borders, then for
 // its state and its last rows.
 //
 // States: the last W-1 inputs of a sequence.  Only the thread that owns a sequence's first token reads the initial state, and it

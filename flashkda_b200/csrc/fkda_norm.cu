@@ -6,9 +6,9 @@
 // One pass: a row lives in the registers of the threads that share it, eight elements (16 bytes of bf16) at a time, from its loads to its
 // stores; the sum of squares is fp32.  Rows of up to 1024 elements are shared by 8 to 32 lanes of a warp, longer ones by a block.
 //
-// Bound by memory: 6 bytes an element (gated), 8 or 12 (residual stream in bf16 or fp32).  4 x 8192 rows of 32 x 128 with their gate take 136 us, 5.9 TB/s:
+// Bound by memory: 6 bytes an element (gated), 8 or 12 (residual stream in bf16 or fp32).  4 x 8192 rows of 32 x 128 with their gate take 142 us, 5.7 TB/s:
 // arithmetic on pairs, and four of these short rows a thread, without which there were too few loads on the way (185 us); 4 x 8192 rows of 4096 with an
-// fp32 residual stream 235 us, 6.9 TB/s.  A step of 64 rows takes 3.5 us, the launch.
+// fp32 residual stream 234 us, 6.9 TB/s.  A step of 64 rows takes 3.3 us, the launch.
 #include "fkda_elem.cuh"
 #include "fkda_layer.cuh"
 

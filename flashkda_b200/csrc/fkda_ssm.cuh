@@ -9,8 +9,9 @@ namespace fkda {
 constexpr int kSsmBlock = 128;       // tokens of a block
 // Sequences of at most this many tokens go token by token (fkda_ssm_step.cu).  Both sides, us, with fp32 states in and out:
 //     heads, P x Ns, batch      32, 64 x 128, 1    32, 64 x 128, 16    32, 64 x 128, 128    32, 128 x 128, 128    32, 64 x 64, 128
-//     16 tokens one by one / in blocks   6.4 / 12.9          25 / 27            144 / 180             278 / 335              75 / 139
-//     32 tokens                         10.7 / 13.0          42 / 28            260 / 183             505 / 339             133 / 141
+//     16 tokens one by one / in blocks   6.2 / 11.8          23 / 24            143 / 161             275 / 315              75 / 136
+//     32 tokens                         10.4 / 11.9          42 / 25            257 / 163             500 / 317             133 / 137
+// (One number for all: a single sequence, and states of 64 x 64, would gain up to 1.5 us in 12 and 4 in 137 from a later border; the others lose far more.)
 constexpr int kSsmStepT = 16;
 constexpr int kSsmPlanMost = 2048;   // packed batches of more sequences keep the given order and are not cut into runs
 // What the planner of runs reckons with, in hundredths of a block's walk (some 3 us): a block of the first pass, what a walk takes beside its

@@ -20,26 +20,31 @@
 //     h = round(x w0),  e = x w0 - h, a bf16 number itself;   two parts: h and round(e + x w1)
 //     three parts: m = round(e + round(x w1));  m - e is a bf16 number too (e is a multiple of the last bit of round(x w1));  l = round(round(x w1 - (m - e)) + x w2)
 // Three instructions for two elements, and seven; taken apart in fp32 it was eight and twelve.  Against 64 bits the final state of 4 x 8192 x 32 x 128 is off by 2.4e-7
-// of its norm with three parts, and would be by 4.7e-6 with two (242 us for 207).
+// of its norm with three parts, and would be by 4.7e-6 with two (240 us for 208); a 32-bit evaluation by products of plain matrices is off by 9e-8.
 // Decays: every exponent that is evaluated is a sum of terms of one sign, so that nothing cancels, but for those within 32 x 32 blocks on
 // the diagonal that lose less than 2^-100: there M's factor is 2^p_i 2^-p_j delta_j, off by 2^-24 of the running sums p, 1e-5 at most.  In blocks that lose
 // more each row adds up its own exponents from the diagonal backwards (a step that resets the state leaves those behind it as they are).
 // Rows past a sequence's end are zeroed in the tiles of x and B where they are summed over; those of C only reach outputs that are not stored.
 //
-// What bounds it (4 x 8192 tokens, 32 heads of P = Ns = 128: 128 CTAs of 64 blocks, 208 us on tensors that are new each time, 180 over and over; 572 MB,
-// 2.7 TB/s; 86 GFLOP as 5 P Ns a token).  Not memory: a block takes 4400 to 4900 cycles, of which its tiles would take 2700.  The products take 2560 of
-// them, all on one chain: M X is done, the output is read out of tensor memory (1100 cycles), C S^T goes there (550), X'^T B (1020), M X (700).  G and C S^T
-// read both operands from shared memory at all that it gives, 128 bytes a cycle, and hold up the other warps' accesses meanwhile.  Left out to see: half
-// of G saves 8 us, the lo part 14, as much as their cycles; reads of x for the output 2, the state's copy and the output's rescaling 1.
+// What bounds it (4 x 8192 tokens, 32 heads of P = Ns = 128: 128 CTAs of 64 blocks, on tensors that are new each time; 86 GFLOP as 5 P Ns a token): 208 us with states
+// in bf16, 2.7 TB/s, 240 in fp32.  Not memory: a block takes 5000 cycles, 5900 with three parts, at the 1.5 to 1.6 GHz that the power limit leaves.  Its chain,
+// traced: X'^T B of the block before is done, the next tile of B comes (1800 cycles; there is room for one), G (700), C S^T (800 to 1000), X'^T B (1040; with three
+// parts 2200, of which its products are 1540); M X (700) and the reading of the output out of tensor memory (900) go beside the way of B.  All of it goes through
+// shared memory: of a block's cycles there the products take 1800 (2050), the warps 1760 (1900), the tensor copies 1000, and G and C S^T read both operands at all that it gives, so that
+// the warps' accesses wait meanwhile.  Left out to see, of 180 us (two parts, the same tensors over and over): half of G 8 us, the second part 14, as much as their cycles;
+// reads of x for the output 2, the state's copy and the output's rescaling 1.
 // Taken: five products of 128 x 128 x 128 on two heads at once, since one head of P = 64 would leave half of a product's rows empty; X'^T in tensor memory
 // (in shared memory: 281 us); a warp a block of M (a table of masks, one copy of the code: unrolled for each kind of block, the kernel no
 // longer fitted in the instruction caches, 10 %).  Taken back: X'^T B before C S^T (the state's warps then wait for C S^T: 186 for 180, packed 435 for 397),
-// the output on warps 8-15 (236), tiles of B and C asked for in the L2 beforehand (none).
+// the output on warps 8-15 (236), tiles of B and C asked for in the L2 beforehand (none).  Of three parts, which tensor memory holds two thirds of at a time (242): parts
+// taken apart in fp32 (250), a quarter of a block at a time (260), the first half before the state's turn (258), M of warps 8-15 between the halves (250) or before the
+// last pieces (251), a token's weights in one word of 16 bytes (255).
 //
-// Few chains are cut into runs (fkda_ssm.cuh): a first pass leaves what each run adds to a zero state, 1.3 us a block, a small launch chains these, and the
-// full pass starts every run from its state.  One sequence of 131072 x 8 heads of 64 takes 164 us (67 ms token by token; 40 us first pass,
-// 8 chaining, 80 full), a prompt of 777 x 32 heads 19.5 us: there each launch's start counts, some 2.5 us until decays and the first tiles are there,
-// so that the launches overlap (see the waits below).  Packed batches of 16 sequences of 256 to 16384 tokens, 32 heads: 434 us, 2.5 TB/s.
+// Few chains are cut into runs (fkda_ssm.cuh): a first pass leaves what each run adds to a zero state, a small launch chains these, and the
+// full pass starts every run from its state.  One sequence of 131072 x 8 heads of 64 takes 167 us with states in bf16 and 188 in fp32 (67 ms token by token): in a trace
+// of such calls the first pass 48 (53), its chaining until 9 behind that, the full pass 92 (103) more.  A prompt of 777 x 32 heads takes 19.1 us (20.4): there each
+// launch's start counts, some 2.5 us until decays and the first tiles are there, so that the launches overlap (see the waits below).  Packed batches of 16 sequences of 256
+// to 16384 tokens, 32 heads: 435 us, 2.5 TB/s (481).
 #include "fkda_elem.cuh"
 #include "fkda_layer.cuh"
 #include "fkda_ssm.cuh"

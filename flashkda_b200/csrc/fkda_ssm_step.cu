@@ -6,7 +6,7 @@
 // four rows with eight columns each, so that a row's product with C folds through four or three shuffles, and B and C are eight
 // registers of a lane.  Rows never meet, so the rows of a state are as many blocks, and a single sequence spreads over the chip.
 //
-// A step is bound by the states, which are read and written: 256 sequences x 32 heads of 64 x 128 in fp32 take 89 us, 6.1 TB/s.  More tokens are bound by
+// A step is bound by the states, which are read and written: 256 sequences x 32 heads of 64 x 128 in fp32 take 89 us, 6.0 TB/s.  More tokens are bound by
 // arithmetic, some 0.5 us a token of an SM's rows, and by what one token takes behind the other, 0.27 us: fkda_ssm.cuh has where the blocks begin.
 #include "fkda_elem.cuh"
 #include "fkda_layer.cuh"

@@ -207,6 +207,7 @@ int fkda_short_conv(const fkda_conv_params* p, void* cuda_stream);
 /* Selective state space scan with one decay per head: with delta = softplus(dt + dt_bias[h]),
  *   S_t = exp(-exp(A_log[h]) delta) S_(t-1) + delta x_t B_t^T,   out_t = S_t C_t + D[h] x_t
  * Heads h * G / H share a group's B and C.  P is 64 or 128, Ns (the columns of a state) 64 or 128, H a multiple of G.
+ * An fp32 final_state is computed to fp32 accuracy, one in bf16 (or none) from states that keep 16 bits of what each token adds, which takes less time.
  * A value that is not finite reaches, beside everything after it, the tokens of its own block of 128 from the sequence's start. */
 typedef struct fkda_ssm_params {
   const void* x;             /* bf16 [B][T][H][P] */
