@@ -4,8 +4,8 @@
 // before the block (per head),
 //     G = C B^T,   M_ij = G_ij 2^(l_i - l_j) delta_j  (j <= i),   out = M X + 2^(l_i) (C S^T) + D X
 //     S <- 2^(l_127) S + X'^T B,   x'_j = 2^(l_127 - l_j) delta_j x_j
-// A CTA walks the blocks of 128 rows of a sequence's states: two heads of P = 64 that share B and C, or one of P = 128.  Five products a block,
-// 128 x 128 x 128 each: G, C S^T, X'^T B twice (X' as hi + lo, below), M X.  Tensor memory holds G and over it M; the output, first as C S^T,
+// A CTA walks the blocks of 128 rows of a sequence's states: two heads of P = 64 that share B and C, or one of P = 128.  Five or six products a block,
+// 128 x 128 x 128 each: G, C S^T, X'^T B in two or three parts (below), M X.  Tensor memory holds G and over it M; the output, first as C S^T,
 // then rescaled by rows, then with M X on top; X'^T; and S.  Twenty warps:
 //     0-15   M from G: a warp a 32 x 32 block (rows i = lanes)
 //     0-7    the output's rescaling (rows i = lanes, half of the columns each warpgroup); then out = that + D x over the tile of x in shared
@@ -33,7 +33,7 @@
 // shared memory: of a block's cycles there the products take 1800 (2050), the warps 1760 (1900), the tensor copies 1000, and G and C S^T read both operands at all that it gives, so that
 // the warps' accesses wait meanwhile.  Left out to see, of 180 us (two parts, the same tensors over and over): half of G 8 us, the second part 14, as much as their cycles;
 // reads of x for the output 2, the state's copy and the output's rescaling 1.
-// Taken: five products of 128 x 128 x 128 on two heads at once, since one head of P = 64 would leave half of a product's rows empty; X'^T in tensor memory
+// Taken: products of 128 x 128 x 128 on two heads at once, since one head of P = 64 would leave half of a product's rows empty; X'^T in tensor memory
 // (in shared memory: 281 us); a warp a block of M (a table of masks, one copy of the code: unrolled for each kind of block, the kernel no
 // longer fitted in the instruction caches, 10 %).  Taken back: X'^T B before C S^T (the state's warps then wait for C S^T: 186 for 180, packed 435 for 397),
 // the output on warps 8-15 (236), tiles of B and C asked for in the L2 beforehand (none).  Of three parts, which tensor memory holds two thirds of at a time (242): parts
@@ -200,7 +200,7 @@ __device__ __forceinline__ void weigh_m(uint32_t (&m)[16], const uint32_t (&g)[3
     m[2 * j + 1] = round2(mul(pk(g[4 * j + 2], g[4 * j + 3]), mul(r2, pk(v.z, v.w))));
   }
 }
-// The block (w, w) where a head forgets.  Apart from make_m, which then is no longer in the instruction caches' way (5 % of a packed batch).
+// The block (w, w) where a head forgets.  Apart from make_m, which then is no longer in the instruction caches' way (in line a packed batch took 465 us where it takes 436).
 template <bool kWide>
 __device__ __noinline__ void make_m_one_by_one(uint32_t at, const Scalars& s, int w, const uint8_t* masks) {
   const int lane = threadIdx.x & 31;
