@@ -108,3 +108,46 @@ def test_a_wait_that_runs_out_with_states_in_bf16(B, T, H, P, lens, stop):
     F.ssm_fwd(*args, workspace=ws)
     assert F.read_status(ws) == 0
     assert torch.equal(out, before) and torch.equal(fin, fin2)
+
+
+@pytest.mark.parametrize("captured", [False, True])
+@pytest.mark.parametrize("state", ["bf16", None])
+@pytest.mark.parametrize("T,P,lens", [(1500, 64, None), (700, 128, None), (20, 64, None), (1, 64, [700, 3, 900, 17])])
+def test_inputs_and_states_in_bf16_that_the_kernel_before_wrote(T, P, lens, state, captured):
+    """The scan's launches overlap: inputs written, a scan, another over the same buffers, again and again, give what each gives alone."""
+    n = T if lens is None else sum(lens)
+    cu = None if lens is None else torch.tensor([0] + torch.tensor(lens).cumsum(0).tolist(), device="cuda")
+    sets = [inputs(1, n, 2, P, 1, 128, seed=s, state=state, N=1 if lens is None else len(lens)) for s in (1, 2)]
+    x, dt, Bm, Cm, A_log, dt_bias, D, x0 = [t.clone() if t is not None else None for t in sets[0]]
+    out = torch.empty_like(x)
+
+    def run():
+        F.ssm_fwd(x, dt, Bm, Cm, out, A_log, dt_bias, D, initial_state=x0, final_state=x0, cu_seqlens=cu)
+        x.copy_(out.clamp(-4, 4))
+        F.ssm_fwd(x, dt, Bm, Cm, out, A_log, dt_bias, D, initial_state=x0, final_state=x0, cu_seqlens=cu)
+
+    def load(s):
+        for to, t in zip((x, dt, Bm, Cm, A_log, dt_bias, D, x0), s):
+            if t is not None:
+                to.copy_(t)
+
+    want = []
+    for s in sets:
+        load(s)
+        torch.cuda.synchronize()
+        run()
+        torch.cuda.synchronize()
+        want.append((out.clone(), x0.clone() if x0 is not None else out))
+    if captured:
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            run()
+    got = []
+    for i in range(10):
+        load(sets[i & 1])
+        graph.replay() if captured else run()
+        got.append((out.clone(), x0.clone() if x0 is not None else want[i & 1][1]))
+    for i, (o, f) in enumerate(got):
+        assert torch.equal(o, want[i & 1][0]) and torch.equal(f, want[i & 1][1])
